@@ -25,7 +25,10 @@ SOURCES = ["conv_mfma.hip", "conv_small.hip", "norm.hip", "gram.hip", "loss.hip"
 ARCH = os.environ.get("RST_OFFLOAD_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-I", str(ROOT / "include"), "-I", str(CSRC),
-          "-Wall", "-Wno-unused-function", "-Wno-unused-variable", "-munsafe-fp-atomics"]
+          "-Wall", "-Wno-unused-function", "-Wno-unused-variable", "-munsafe-fp-atomics",
+          # no packed FP32 (v_pk_*_f32): some of its forms gave wrong sums beside other waves of the CU. Costs the frame
+          # 0.65 % (1667 -> 1656 FPS, two alternating pairs), the training step nothing (20.1-20.4 ms)
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 # per-source extra flags: the split-bf16 Winograd kernel keeps its transform in scalar f32 ops (packed f32
