@@ -20,6 +20,10 @@
  *                                                                 predict_video_using_checkpoint.py:96
  *   rst_gram                     gram_matrix / get_gram_matrix_model  models/styleLoss.py:11-37
  *   rst_instance_norm            ConditionalInstanceNormalization.call models/styleTransfer.py:57-71
+ *   rst_group_norm               no reference counterpart: group normalisation with an activation, forward and backward,
+ *                                next to rst_instance_norm (its groups == channels case)
+ *   rst_adamw_*                  no reference counterpart: the AdamW step over many tensors, beside the trainers'
+ *                                RMSprop (train_network.py:102)
  *   rst_copy_activation          (debug) per-block outputs of the Keras sub-models
  *   rst_predictor_*              create_style_prediction_model(input_shape, feature_extractor,
  *                                num_top_parameters, num_style_parameters=100) -> tf.keras.Model
@@ -144,6 +148,26 @@ size_t rst_instance_norm_workspace_size(int batch, int hw, int channels);
 int rst_instance_norm(const float* x, int batch, int hw, int channels, const float* scale, const float* bias,
                       float eps, int relu, float* y, void* workspace, void* stream);
 
+/* ---- Group normalisation with an activation (channels last) ----
+ * x (B, hw, C), `groups` groups of C / groups channels; per (b, group): mean and (biased) variance over hw and the group's
+ * channels, rstd = 1 / sqrt(var + eps), y = act(scale_c (x - mean) rstd + bias_c). x, y, dy and dx are `dtype`
+ * (RST_DTYPE_*), everything else f32. scale / bias: (C), or (B, C) with per_image != 0 (style parameters). Any C, any
+ * number of groups that divides it, any alignment of the element type; 16-byte alignment with C a multiple of 16 bytes
+ * runs on 16-byte loads. y may be x. mean / rstd (B, groups) receive the statistics when not NULL.
+ * backward: from dy, x and the forward's mean / rstd: dx (may be dy), dscale and dbias shaped as scale / bias (sums over
+ * the batch where they are shared). The same inputs give the same bits (no atomics). batch or hw 0: RST_OK, nothing is
+ * written but dscale = dbias = 0. workspace: rst_group_norm_workspace_size() bytes, aligned to 16, used by one call at a
+ * time (calls on two streams, or two captured graphs that may replay together, need one each). */
+enum { RST_DTYPE_FLOAT32 = 0, RST_DTYPE_BFLOAT16 = 1 };
+enum { RST_ACT_LINEAR = 0, RST_ACT_RELU = 1, RST_ACT_SWISH = 2, RST_ACT_HARD_SWISH = 3 };
+size_t rst_group_norm_workspace_size(int batch, int hw, int channels, int groups);
+int rst_group_norm(const void* x, int dtype, int batch, int hw, int channels, int groups, const float* scale,
+                   const float* bias, int per_image, float eps, int activation, void* y, float* mean, float* rstd,
+                   void* workspace, void* stream);
+int rst_group_norm_backward(const void* x, const void* dy, int dtype, int batch, int hw, int channels, int groups,
+                            const float* scale, const float* bias, int per_image, const float* mean, const float* rstd,
+                            int activation, void* dx, float* dscale, float* dbias, void* workspace, void* stream);
+
 /* ---- VGG16 / Gram style loss (StyleLossModelVGG + make_style_loss_function, no depth term) ---- */
 typedef struct rst_loss_shape {
     int h, w;                 /* prediction / content / style image size (multiples of 16)        */
@@ -227,6 +251,10 @@ int rst_trainer_wait_style_gradient(rst_trainer* t, void* stream);
  * into the kernels' weight images. Keras defaults: lr 1e-3, rho 0.9, epsilon 1e-7. */
 int rst_trainer_apply_gradients(rst_trainer* t, const float* grad, float learning_rate, float rho, float epsilon,
                                 void* stream);
+/* For an optimizer other than RMSprop: the trainer's own device-resident weights (Keras order, owned by t), to be
+ * updated in place on a stream, and the re-pack of the kernels' weight images that has to follow on that stream. */
+float* rst_trainer_weights(rst_trainer* t);
+int rst_trainer_weights_updated(rst_trainer* t, void* stream);
 /* Device copies of the current weights (Keras order) / RMSprop slots; set_weights re-packs. */
 int rst_trainer_copy_weights(rst_trainer* t, float* dst, size_t count, void* stream);
 int rst_trainer_copy_slots(rst_trainer* t, float* dst, size_t count, void* stream);
@@ -300,6 +328,7 @@ int rst_predictor_trainer_forward(rst_predictor_trainer* t, const float* style, 
 int rst_predictor_trainer_backward(rst_predictor_trainer* t, const float* d_style_params, float* grad, void* stream);
 int rst_predictor_trainer_apply_gradients(rst_predictor_trainer* t, const float* grad, float learning_rate, float rho,
                                           float epsilon, void* stream);
+float* rst_predictor_trainer_weights(rst_predictor_trainer* t);   /* as rst_trainer_weights; nothing to re-pack */
 int rst_predictor_trainer_copy_weights(rst_predictor_trainer* t, float* dst, size_t count, void* stream);
 int rst_predictor_trainer_set_weights(rst_predictor_trainer* t, const float* src, size_t count, void* stream);
 int rst_predictor_trainer_copy_slots(rst_predictor_trainer* t, float* dst, size_t count, void* stream);
@@ -309,6 +338,53 @@ size_t rst_predictor_trainer_num_moving_statistics(const rst_predictor_trainer* 
 int rst_predictor_trainer_get_moving_statistics(rst_predictor_trainer* t, float* dst, size_t count, void* stream);
 int rst_predictor_trainer_set_moving_statistics(rst_predictor_trainer* t, const float* src, size_t count, float divisor,
                                                 void* stream);
+
+/* ---- AdamW over many tensors ----
+ * One step t for all variables, with c = min(1, global_clipnorm / |g|) over all of them (1 without clipping):
+ *   m = beta_1 m + (1 - beta_1) c g;  v = beta_2 v + (1 - beta_2) (c g)^2
+ *   p -= learning_rate (m / (1 - beta_1^t) / (sqrt(v / (1 - beta_2^t)) + epsilon) + weight_decay p)
+ * weight_decay applies to the variables created with decay != 0. Variables are f32 device memory at any float; gradients
+ * (f32 or bf16) come in one bucket, variable k's at element grad_offset of it, or one tensor per variable.
+ * State, caller-owned device memory that must outlive the handle:
+ *   state_bits 32: m, v f32, the variables' elements one after the other (no gaps).
+ *   state_bits 8: m, v e4m3 codes in blocks of 128 elements of one variable, the variables' blocks one after the other
+ *     (a variable's last block is filled with zeros), aligned to 8 bytes; m_scale, v_scale one f32 per block. A state
+ *     is code * scale, scale = max / 448. m / scale rounds to nearest; v / scale rounds up or down at random with the
+ *     right mean (bits from a hash of the element, the step and `seed`), never from above zero to zero. The step uses
+ *     the m and v before they are rounded.
+ *   iterations: steps taken (t = iterations + 1), moved on by every step on the device: a captured step replays as the
+ *     next one. Hyperparameters are captured by value.
+ *   global_norm: receives |g| of each step that clips (may be NULL). If |g| is not finite that step changes nothing,
+ *     iterations included. Without clipping a NaN or infinity spreads as the formula says (with 8 bits: to its block).
+ * States start as zeros (iterations 0). One step of a handle at a time: not on two streams at once. */
+typedef struct rst_adamw_tensor {
+    float* param;
+    size_t count;
+    size_t grad_offset;      /* element of the gradient bucket (rst_adamw_step) */
+    int decay;               /* weight_decay applies */
+} rst_adamw_tensor;
+typedef struct rst_adamw_state {
+    void* m;
+    void* v;
+    float* m_scale;          /* state_bits 8 */
+    float* v_scale;
+    long long* iterations;
+    float* global_norm;
+} rst_adamw_state;
+typedef struct rst_adamw_config {
+    double learning_rate, weight_decay, beta_1, beta_2, epsilon;
+    double global_clipnorm;  /* 0: no clipping */
+    unsigned seed;           /* of the 8-bit rounding */
+} rst_adamw_config;
+typedef struct rst_adamw rst_adamw;
+int rst_adamw_create(const rst_adamw_tensor* tensors, int num_tensors, int state_bits, const rst_adamw_state* state,
+                     rst_adamw** out);
+void rst_adamw_destroy(rst_adamw* h);
+size_t rst_adamw_num_blocks(const rst_adamw* h);
+/* gradients: the bucket (device). _tensors: HOST array of one device pointer per variable, in creation order. */
+int rst_adamw_step(rst_adamw* h, const void* gradients, int dtype, const rst_adamw_config* config, void* stream);
+int rst_adamw_step_tensors(rst_adamw* h, const void* const* gradients, int num_tensors, int dtype,
+                           const rst_adamw_config* config, void* stream);
 
 /* ---- G-buffer ingest ----
  * Replaces the host-side numpy/TF preprocessing of an Unreal HDR screenshot:

@@ -25,6 +25,9 @@ EXPORTED_SYMBOLS = [
     "rst_create", "rst_create_ex", "rst_precision", "rst_destroy", "rst_num_style_params", "rst_num_weights_for_shape", "rst_forward",
     "rst_num_layers", "rst_layer_output_shape", "rst_copy_activation", "rst_gram_workspace_size", "rst_gram",
     "rst_instance_norm_workspace_size", "rst_instance_norm", "rst_style_param_map", "rst_last_error", "rst_version",
+    "rst_group_norm_workspace_size", "rst_group_norm", "rst_group_norm_backward",
+    "rst_adamw_create", "rst_adamw_destroy", "rst_adamw_num_blocks", "rst_adamw_step", "rst_adamw_step_tensors",
+    "rst_trainer_weights", "rst_trainer_weights_updated", "rst_predictor_trainer_weights",
     "rst_profile_begin", "rst_profile_end", "rst_timeline_begin", "rst_timeline_read", "rst_timeline_end",
     "rst_layer_kernel_id",
     "rst_loss_num_weights", "rst_loss_create", "rst_loss_destroy", "rst_loss_forward", "rst_loss_copy_feature",
@@ -44,6 +47,8 @@ EXPORTED_SYMBOLS = [
     "rst_predictor_trainer_set_moving_statistics",
     "rst_gbuffer_resized_size", "rst_gbuffer_preprocess", "rst_crc32c_extend",
 ]
+DTYPES = {"float32": 0, "bfloat16": 1}       # include/rst.h RST_DTYPE_*
+ACTIVATIONS = {"linear": 0, "relu": 1, "swish": 2, "hard_swish": 3}   # include/rst.h RST_ACT_*
 EXTRACTORS = {"DUMMY": 0, "MOBILE_NET": 1}   # include/rst.h RST_EXTRACTOR_*
 
 
@@ -64,6 +69,20 @@ class RstPredictorShape(ctypes.Structure):
     _fields_ = [("h", ctypes.c_int), ("w", ctypes.c_int), ("c", ctypes.c_int), ("feature_extractor", ctypes.c_int),
                 ("num_top_parameters", ctypes.c_int), ("num_style_parameters", ctypes.c_int),
                 ("max_batch", ctypes.c_int)]
+
+
+class RstAdamwTensor(ctypes.Structure):
+    _fields_ = [("param", ctypes.c_void_p), ("count", ctypes.c_size_t), ("grad_offset", ctypes.c_size_t),
+                ("decay", ctypes.c_int)]
+
+
+class RstAdamwState(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("m", "v", "m_scale", "v_scale", "iterations", "global_norm")]
+
+
+class RstAdamwConfig(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_double) for n in ("learning_rate", "weight_decay", "beta_1", "beta_2", "epsilon",
+                                               "global_clipnorm")] + [("seed", ctypes.c_uint)]
 
 
 class RstError(RuntimeError):
@@ -139,6 +158,29 @@ def load() -> ctypes.CDLL:
     lib.rst_instance_norm.restype = i
     lib.rst_style_param_map.argtypes = [vp, vp, i, i, i, i, vp, vp]
     lib.rst_style_param_map.restype = i
+    lib.rst_group_norm_workspace_size.argtypes = [i, i, i, i]
+    lib.rst_group_norm_workspace_size.restype = sz
+    lib.rst_group_norm.argtypes = [vp, i, i, i, i, i, vp, vp, i, fp, i, vp, vp, vp, vp, vp]
+    lib.rst_group_norm.restype = i
+    lib.rst_group_norm_backward.argtypes = [vp, vp, i, i, i, i, i, vp, vp, i, vp, vp, i, vp, vp, vp, vp, vp]
+    lib.rst_group_norm_backward.restype = i
+    lib.rst_adamw_create.argtypes = [ctypes.POINTER(RstAdamwTensor), i, i, ctypes.POINTER(RstAdamwState),
+                                     ctypes.POINTER(vp)]
+    lib.rst_adamw_create.restype = i
+    lib.rst_adamw_destroy.argtypes = [vp]
+    lib.rst_adamw_destroy.restype = None
+    lib.rst_adamw_num_blocks.argtypes = [vp]
+    lib.rst_adamw_num_blocks.restype = sz
+    lib.rst_adamw_step.argtypes = [vp, vp, i, ctypes.POINTER(RstAdamwConfig), vp]
+    lib.rst_adamw_step.restype = i
+    lib.rst_adamw_step_tensors.argtypes = [vp, ctypes.POINTER(vp), i, i, ctypes.POINTER(RstAdamwConfig), vp]
+    lib.rst_adamw_step_tensors.restype = i
+    lib.rst_trainer_weights.argtypes = [vp]
+    lib.rst_trainer_weights.restype = vp
+    lib.rst_trainer_weights_updated.argtypes = [vp, vp]
+    lib.rst_trainer_weights_updated.restype = i
+    lib.rst_predictor_trainer_weights.argtypes = [vp]
+    lib.rst_predictor_trainer_weights.restype = vp
     lib.rst_profile_begin.argtypes = [vp, i]
     lib.rst_profile_begin.restype = i
     lib.rst_profile_end.argtypes = [vp, ctypes.POINTER(fp), ctypes.POINTER(fp), ctypes.POINTER(i)]

@@ -1,0 +1,187 @@
+// adamw_api.hip — C ABI of the AdamW step over many tensors (include/rst.h rst_adamw_*).
+//
+// rst_adamw_create cuts the variables into chunks once and keeps the table on the device; a step is then one launch
+// (three with global-norm clipping and separate gradient tensors: pointers, norm, step). Nothing is allocated or
+// synchronised by a step.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "../../include/rst.h"
+#include "adamw.h"
+#include "common.h"
+
+using namespace rst;
+
+struct rst_adamw {
+    int device = 0, bits = 32, num_tensors = 0, num_chunks = 0;
+    size_t num_blocks = 0, num_elements = 0;
+    rst_adamw_state state{};
+    AdamwChunk* d_chunks = nullptr;
+    const void** d_ptrs = nullptr;
+    double* d_partials = nullptr;
+    unsigned* d_ticket = nullptr;
+    ~rst_adamw() {
+        (void)hipFree(d_chunks);
+        (void)hipFree(d_ptrs);
+        (void)hipFree(d_partials);
+        (void)hipFree(d_ticket);
+    }
+};
+
+namespace {
+
+int step_args(rst_adamw* h, const char* who, int dtype, const rst_adamw_config* c, AdamwArgs& a) {
+    const std::string name(who);
+    if (dtype != RST_DTYPE_FLOAT32 && dtype != RST_DTYPE_BFLOAT16)
+        return set_error(RST_ERR_UNSUPPORTED, name + ": gradients are float32 or bfloat16");
+    if (!(c->beta_1 >= 0.0 && c->beta_1 < 1.0 && c->beta_2 >= 0.0 && c->beta_2 < 1.0))
+        return set_error(RST_ERR_INVALID, name + ": beta_1 and beta_2 must lie in [0, 1)");
+    if (!std::isfinite(c->learning_rate) || !std::isfinite(c->weight_decay) || !(c->epsilon >= 0.0) ||
+        !std::isfinite(c->epsilon) || !(c->global_clipnorm >= 0.0))
+        return set_error(RST_ERR_INVALID, name + ": hyperparameters must be finite, epsilon and global_clipnorm not negative");
+    int dev = 0;
+    RST_HIP_TRY(hipGetDevice(&dev));
+    if (dev != h->device)
+        return set_error(RST_ERR_INVALID, name + ": made on device " + std::to_string(h->device) +
+                                              ", called on device " + std::to_string(dev));
+    a.chunks = h->d_chunks;
+    a.grad_ptrs = h->d_ptrs;
+    a.grad_bf16 = dtype == RST_DTYPE_BFLOAT16;
+    a.num_chunks = h->num_chunks;
+    a.m = h->state.m;
+    a.v = h->state.v;
+    a.m_scale = h->state.m_scale;
+    a.v_scale = h->state.v_scale;
+    a.iterations = h->state.iterations;
+    a.global_norm = h->state.global_norm;
+    a.ticket = h->d_ticket;
+    a.partials = h->d_partials;
+    a.num_partials = c->global_clipnorm > 0.0 ? std::min(h->num_chunks, ADAMW_MAX_PARTIALS) : 0;
+    a.lr = c->learning_rate;
+    a.decay = c->weight_decay;
+    a.b1 = c->beta_1;
+    a.b2 = c->beta_2;
+    a.eps = c->epsilon;
+    a.clip = c->global_clipnorm;
+    a.log_b1 = std::log(c->beta_1);
+    a.log_b2 = std::log(c->beta_2);
+    a.seed = c->seed;
+    return RST_OK;
+}
+
+int launch(rst_adamw* h, const AdamwArgs& a, hipStream_t st) {
+    if (h->num_chunks == 0) return RST_OK;
+    if (a.num_partials > 0) RST_HIP_TRY(adamw_norm_launch(a, h->d_partials, st));
+    RST_HIP_TRY(adamw_step_launch(a, h->bits, st));
+    return RST_OK;
+}
+
+int create(const rst_adamw_tensor* tensors, int n, int bits, const rst_adamw_state* state, rst_adamw* h) {
+    std::vector<AdamwChunk> chunks;
+    size_t blocks = 0, elements = 0;
+    for (int k = 0; k < n; ++k) {
+        const rst_adamw_tensor& t = tensors[k];
+        if (t.count != 0 && t.param == nullptr) return set_error(RST_ERR_INVALID, "rst_adamw_create: null variable");
+        if (t.count > ((size_t)1 << 40)) return set_error(RST_ERR_INVALID, "rst_adamw_create: variable too large");
+        for (size_t i = 0; i < t.count; i += ADAMW_CHUNK) {
+            AdamwChunk c{};
+            c.param = t.param + i;
+            c.grad_at = (long long)(t.grad_offset + i);
+            c.tensor_at = (long long)i;
+            c.state_at = (long long)(bits == 8 ? blocks * ADAMW_BLOCK + i : elements + i);
+            c.count = (int)std::min((size_t)ADAMW_CHUNK, t.count - i);
+            c.tensor = k;
+            c.decay = t.decay != 0;
+            chunks.push_back(c);
+        }
+        blocks += (t.count + ADAMW_BLOCK - 1) / ADAMW_BLOCK;
+        elements += t.count;
+    }
+    if (chunks.size() >= (size_t)1 << 31) return set_error(RST_ERR_UNSUPPORTED, "rst_adamw_create: too many elements");
+    if (elements != 0 && (state->m == nullptr || state->v == nullptr ||
+                          (bits == 8 && (state->m_scale == nullptr || state->v_scale == nullptr))))
+        return set_error(RST_ERR_INVALID, "rst_adamw_create: null state");
+    if (bits == 8 && (((size_t)state->m | (size_t)state->v) & 7) != 0)
+        return set_error(RST_ERR_INVALID, "rst_adamw_create: 8-bit states must be aligned to 8 bytes");
+    RST_HIP_TRY(hipGetDevice(&h->device));
+    h->bits = bits;
+    h->num_tensors = n;
+    h->num_chunks = (int)chunks.size();
+    h->num_blocks = blocks;
+    h->num_elements = elements;
+    h->state = *state;
+    if (chunks.empty()) return RST_OK;
+    const unsigned zero = 0;
+    if (hipMalloc(&h->d_chunks, chunks.size() * sizeof(AdamwChunk)) != hipSuccess ||
+        hipMalloc(&h->d_ptrs, n * sizeof(void*)) != hipSuccess ||
+        hipMalloc(&h->d_partials, ADAMW_MAX_PARTIALS * sizeof(double)) != hipSuccess ||
+        hipMalloc(&h->d_ticket, sizeof(unsigned)) != hipSuccess)
+        return set_error(RST_ERR_ALLOC, "rst_adamw_create: device allocation failed");
+    RST_HIP_TRY(hipMemcpy(h->d_chunks, chunks.data(), chunks.size() * sizeof(AdamwChunk), hipMemcpyHostToDevice));
+    RST_HIP_TRY(hipMemcpy(h->d_ticket, &zero, sizeof(zero), hipMemcpyHostToDevice));
+    return RST_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rst_adamw_create(const rst_adamw_tensor* tensors, int num_tensors, int state_bits, const rst_adamw_state* state,
+                     rst_adamw** out) {
+    if (tensors == nullptr || state == nullptr || out == nullptr || num_tensors <= 0 || state->iterations == nullptr)
+        return set_error(RST_ERR_INVALID, "rst_adamw_create: bad argument");
+    if (state_bits != 8 && state_bits != 32)
+        return set_error(RST_ERR_UNSUPPORTED, "rst_adamw_create: state_bits must be 8 or 32");
+    *out = nullptr;
+    rst_adamw* h = nullptr;
+    int rc;
+    try {
+        h = new rst_adamw;
+        rc = create(tensors, num_tensors, state_bits, state, h);
+    } catch (const std::exception&) {
+        rc = set_error(RST_ERR_ALLOC, "rst_adamw_create: out of host memory");
+    }
+    if (rc != RST_OK) {
+        delete h;
+        return rc;
+    }
+    *out = h;
+    return RST_OK;
+}
+
+void rst_adamw_destroy(rst_adamw* h) { delete h; }
+
+size_t rst_adamw_num_blocks(const rst_adamw* h) { return h ? h->num_blocks : 0; }
+
+int rst_adamw_step(rst_adamw* h, const void* gradients, int dtype, const rst_adamw_config* config, void* stream) {
+    if (h == nullptr || config == nullptr || (gradients == nullptr && h->num_chunks != 0))
+        return set_error(RST_ERR_INVALID, "rst_adamw_step: null argument");
+    AdamwArgs a{};
+    const int rc = step_args(h, "rst_adamw_step", dtype, config, a);
+    if (rc != RST_OK) return rc;
+    a.bucket = gradients;
+    return launch(h, a, static_cast<hipStream_t>(stream));
+}
+
+int rst_adamw_step_tensors(rst_adamw* h, const void* const* gradients, int num_tensors, int dtype,
+                           const rst_adamw_config* config, void* stream) {
+    if (h == nullptr || config == nullptr || gradients == nullptr || num_tensors != h->num_tensors)
+        return set_error(RST_ERR_INVALID, "rst_adamw_step_tensors: null argument, or not one gradient per variable");
+    AdamwArgs a{};
+    const int rc = step_args(h, "rst_adamw_step_tensors", dtype, config, a);
+    if (rc != RST_OK) return rc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (h->num_chunks != 0)
+        for (int k = 0; k < num_tensors; k += ADAMW_PTRS) {
+            AdamwPtrs p{};
+            const int n = std::min(ADAMW_PTRS, num_tensors - k);
+            std::copy(gradients + k, gradients + k + n, p.p);
+            RST_HIP_TRY(adamw_set_pointers_launch(p, h->d_ptrs + k, n, st));
+        }
+    return launch(h, a, st);
+}
+
+}  // extern "C"

@@ -471,6 +471,8 @@ int rst_predictor_trainer_apply_gradients(rst_predictor_trainer* t, const float*
     return RST_OK;
 }
 
+float* rst_predictor_trainer_weights(rst_predictor_trainer* t) { return t ? t->d_wc : nullptr; }
+
 int rst_predictor_trainer_copy_weights(rst_predictor_trainer* t, float* dst, size_t count, void* stream) {
     if (!t || !dst || count != t->plan.total) return set_error(RST_ERR_INVALID, "rst_predictor_trainer_copy_weights");
     RST_HIP_TRY(hipMemcpyAsync(dst, t->d_wc, count * 4, hipMemcpyDeviceToDevice, (hipStream_t)stream));

@@ -27,6 +27,7 @@
 
 #include "../../include/rst.h"
 #include "common.h"
+#include "group_norm.h"
 #include "kernels.h"
 #include "net.h"
 
@@ -1109,6 +1110,85 @@ int rst_instance_norm(const float* x, int batch, int hw, int channels, const flo
     f.eps = eps;
     HIP_TRY(finalize_launch(f, st));
     HIP_TRY(affine_act_launch(x, ab, nullptr, y, batch, hw, channels, relu ? 1 : 0, st));
+    return RST_OK;
+}
+
+size_t rst_group_norm_workspace_size(int batch, int hw, int channels, int groups) {
+    return group_norm_workspace_bytes(batch, hw, channels, groups);
+}
+
+static int group_norm_check(const char* who, int dtype, int batch, int hw, int channels, int groups, int activation) {
+    const std::string name(who);
+    if (batch < 0 || hw < 0 || channels <= 0 || groups <= 0 || channels % groups != 0)
+        return fail(RST_ERR_INVALID, name + ": batch and hw must not be negative, groups must divide the channels");
+    if (dtype != RST_DTYPE_FLOAT32 && dtype != RST_DTYPE_BFLOAT16)
+        return fail(RST_ERR_UNSUPPORTED, name + ": tensors are float32 or bfloat16");
+    if (activation < RST_ACT_LINEAR || activation > RST_ACT_HARD_SWISH)
+        return fail(RST_ERR_UNSUPPORTED, name + ": unknown activation");
+    if (!group_norm_supported(batch, hw, channels, groups))
+        return fail(RST_ERR_UNSUPPORTED, name + ": too many workgroups for one launch");
+    return RST_OK;
+}
+
+int rst_group_norm(const void* x, int dtype, int batch, int hw, int channels, int groups, const float* scale,
+                   const float* bias, int per_image, float eps, int activation, void* y, float* mean, float* rstd,
+                   void* workspace, void* stream) {
+    const int rc = group_norm_check("rst_group_norm", dtype, batch, hw, channels, groups, activation);
+    if (rc != RST_OK) return rc;
+    if (batch == 0 || hw == 0) return RST_OK;
+    if (x == nullptr || scale == nullptr || bias == nullptr || y == nullptr || workspace == nullptr ||
+        ((size_t)workspace & 15) != 0 || !(eps >= 0.f))
+        return fail(RST_ERR_INVALID, "rst_group_norm: null pointer, workspace not aligned to 16 bytes or negative eps");
+    GroupNormArgs a{};
+    a.x = x;
+    a.out = y;
+    a.scale = scale;
+    a.bias = bias;
+    a.aff_stride = per_image ? channels : 0;
+    a.mean = mean;
+    a.rstd = rstd;
+    a.workspace = workspace;
+    a.hw = hw;
+    a.batch = batch;
+    a.C = channels;
+    a.G = groups;
+    a.eps = eps;
+    a.act = activation;
+    a.bf16 = dtype == RST_DTYPE_BFLOAT16;
+    HIP_TRY(group_norm_launch(a, static_cast<hipStream_t>(stream)));
+    return RST_OK;
+}
+
+int rst_group_norm_backward(const void* x, const void* dy, int dtype, int batch, int hw, int channels, int groups,
+                            const float* scale, const float* bias, int per_image, const float* mean, const float* rstd,
+                            int activation, void* dx, float* dscale, float* dbias, void* workspace, void* stream) {
+    const int rc = group_norm_check("rst_group_norm_backward", dtype, batch, hw, channels, groups, activation);
+    if (rc != RST_OK) return rc;
+    const bool empty = batch == 0 || hw == 0;
+    if (dscale == nullptr || dbias == nullptr)
+        return fail(RST_ERR_INVALID, "rst_group_norm_backward: null pointer");
+    if (!empty && (x == nullptr || dy == nullptr || scale == nullptr || bias == nullptr || mean == nullptr ||
+                   rstd == nullptr || dx == nullptr || workspace == nullptr || ((size_t)workspace & 15) != 0))
+        return fail(RST_ERR_INVALID, "rst_group_norm_backward: null pointer or workspace not aligned to 16 bytes");
+    GroupNormArgs a{};
+    a.x = x;
+    a.dy = dy;
+    a.out = dx;
+    a.scale = scale;
+    a.bias = bias;
+    a.aff_stride = per_image ? channels : 0;
+    a.mean = const_cast<float*>(mean);
+    a.rstd = const_cast<float*>(rstd);
+    a.dscale = dscale;
+    a.dbias = dbias;
+    a.workspace = workspace;
+    a.hw = hw;
+    a.batch = batch;
+    a.C = channels;
+    a.G = groups;
+    a.act = activation;
+    a.bf16 = dtype == RST_DTYPE_BFLOAT16;
+    HIP_TRY(group_norm_bwd_launch(a, static_cast<hipStream_t>(stream)));
     return RST_OK;
 }
 

@@ -1089,6 +1089,13 @@ int rst_trainer_apply_gradients(rst_trainer* t, const float* grad, float learnin
     return repack(t, st);
 }
 
+float* rst_trainer_weights(rst_trainer* t) { return t ? t->d_wc : nullptr; }
+
+int rst_trainer_weights_updated(rst_trainer* t, void* stream) {
+    if (!t) return set_error(RST_ERR_INVALID, "rst_trainer_weights_updated: null handle");
+    return repack(t, static_cast<hipStream_t>(stream));
+}
+
 int rst_trainer_copy_weights(rst_trainer* t, float* dst, size_t count, void* stream) {
     if (!t || !dst || count != t->nw) return set_error(RST_ERR_INVALID, "rst_trainer_copy_weights: bad argument");
     RST_HIP_TRY(hipMemcpyAsync(dst, t->d_wc, count * 4, hipMemcpyDeviceToDevice, static_cast<hipStream_t>(stream)));

@@ -34,6 +34,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .optimizers import AdamW
 from .plan import Plan, init_weights, network_plan
 from .styleLoss import DEPTH_LOSS_UNAVAILABLE, StyleLossModelVGG, make_style_loss_function
 from .styleTransfer import StyleTransferModel
@@ -41,6 +42,7 @@ from .styleTransferInferenceModel import StyleTransferInference, make_style_tran
 
 log = logging.getLogger(__name__)
 
+_ADAMW_HYPER = ('learning_rate', 'weight_decay', 'beta_1', 'beta_2')      # of a checkpoint, beside ``iter``
 LOSS_NAMES = ('loss', 'feature_loss', 'style_loss', 'total_variation_loss')
 
 
@@ -107,7 +109,7 @@ class StyleTransferTrainingModel:
 
     def __init__(self, input_shape, output_shape, bottleneck_res_y, bottleneck_num_filters,
                  loss_model: Optional[StyleLossModelVGG] = None, weights: Optional[Sequence[np.ndarray]] = None,
-                 seed: int = 2, max_batch: int = 4, optimizer: Optional[RMSprop] = None, process_group=None,
+                 seed: int = 2, max_batch: int = 4, optimizer=None, process_group=None,
                  device=None, name: str = "StyleTransferTrainingModel", style_predictor=None,
                  precision: str = "winograd_bf16x6", with_depth_loss: bool = False):
         """``loss_model``: a StyleLossModelVGG (trainable), or a construct-only loss model such as
@@ -115,6 +117,7 @@ class StyleTransferTrainingModel:
         ``train_step`` raises — what the reference's inference and export scripts need
         (predict_video_using_checkpoint.py:43-58, save_using_checkpoint.py:39-53). ``with_depth_loss``: the
         loss asked for the MiDaS depth term (unavailable): construction works, ``train_step`` raises.
+        ``optimizer``: an ``RMSprop`` (default) or an ``optimizers.AdamW``.
         ``precision``: the transfer network's arithmetic — "winograd_bf16x6" (default; fp32-level, the benchmarked
         config-4 line), "fp32_winograd" or "fp32"; the VGG16 loss network's comes from ``loss_model.precision``."""
         if precision not in ("fp32", "fp32_winograd", "winograd_bf16x6"):
@@ -195,8 +198,36 @@ class StyleTransferTrainingModel:
             attrs = ['kernel', 'bias'] + (['gamma', 'beta', 'moving_mean', 'moving_variance'] if layer.norm == 'bn' else [])
             named += list(zip(attrs, layer.weight_shapes))
         self._bn_index = torch.from_numpy(moving_statistics_index(named)).to(self.device)
+        self._trainable = [not name.startswith('moving_') for name, _ in named]
         self._grad = self._bucket[:self.num_weights]
         self._pgrad = self._bucket[self.num_weights:nb] if n_pred else None
+        self._bind_optimizer()
+
+    def _bind_optimizer(self):
+        """Give an AdamW the trainable weights of both networks: device memory of the trainers, each weight's gradient
+        at its place in the bucket (the BN moving statistics between them have none). Kernels decay, biases and norm
+        affines do not."""
+        if not isinstance(self.optimizer, AdamW):
+            return
+        lib, pr = _lib.load(), self.style_predictor
+        groups = [(lib.rst_trainer_weights(self._handle), 0, self._trainable, self._shapes)]
+        if pr is not None:
+            from .stylePrediction import trainable_mask
+            groups.append((lib.rst_predictor_trainer_weights(pr._handle), self.num_weights, trainable_mask(pr.spec),
+                           pr._shapes))
+        pointers, counts, offsets, decay = [], [], [], []
+        for base, first, trainable, shapes in groups:
+            o = 0
+            for train, shape in zip(trainable, shapes):
+                n = int(np.prod(shape))
+                if train:
+                    pointers.append(base + 4 * o)
+                    counts.append(n)
+                    offsets.append(first + o)
+                    decay.append(len(shape) > 1)
+                o += n
+        self.optimizer._build(pointers, counts, offsets, decay, self.device, owner=self)
+        self.optimizer._bucket_size = self._grad_bucket.numel()
 
     # ------------------------------------------------------------------ lifecycle
     def _flatten(self, weights: Sequence[np.ndarray]) -> np.ndarray:
@@ -274,15 +305,24 @@ class StyleTransferTrainingModel:
     trainable = True
 
     def compile(self, run_eagerly=False, optimizer=None, **kwargs):
-        """Keras Model.compile (train_network.py:103-106): takes the optimizer (an RMSprop of this module)."""
-        if optimizer is not None:
-            if not isinstance(optimizer, RMSprop):
+        """Keras Model.compile (train_network.py:103-106): takes the optimizer, an RMSprop of this module (the
+        reference's, train_network.py:102) or an ``optimizers.AdamW``, which steps both networks at once."""
+        if optimizer is not None and optimizer is not self.optimizer:
+            if not isinstance(optimizer, (RMSprop, AdamW)):
                 raise TypeError("optimizer must be styleTransferTrainingModel.RMSprop (the reference's only optimizer, "
-                                "train_network.py:102)")
-            self.optimizer = optimizer
+                                "train_network.py:102) or optimizers.AdamW")
+            before, self.optimizer = self.optimizer, optimizer
+            if self._handle is not None:
+                try:
+                    self._bind_optimizer()
+                except BaseException:
+                    self.optimizer = before
+                    raise
 
     def optimizer_slots(self) -> List[np.ndarray]:
-        """RMSprop ``rms`` slots in weight order."""
+        """RMSprop ``rms`` slots in weight order (an AdamW's moments: ``optimizer.slots()``)."""
+        if isinstance(self.optimizer, AdamW):
+            raise ValueError("optimizer_slots are RMSprop's: an AdamW keeps its moments, optimizer.slots()")
         t = torch.empty(self.num_weights, dtype=torch.float32, device=self.device)
         _lib.check(_lib.load().rst_trainer_copy_slots(self._handle, _lib.dev_ptr(t), t.numel(), _lib.stream_ptr()))
         return self._unflatten(t.cpu().numpy())
@@ -326,10 +366,29 @@ class StyleTransferTrainingModel:
             groups.insert(0, (parts[0], trainable_mask(pr.spec), pr.optimizer_slots, pr.set_optimizer_slots))
         return groups
 
+    def _adamw_paths(self):
+        """The checkpoint paths of an AdamW's variables, in its order, and their shapes."""
+        from .stylePrediction import trainable_mask
+        parts = self._checkpoint_parts()
+        masks = ([trainable_mask(self.style_predictor.spec)] if self.style_predictor is not None else []) + [self._trainable]
+        named = [[(path, shape) for path, shape, train in zip(part.tree.paths(part.prefix), shapes, mask) if train]
+                 for part, shapes, mask in zip(parts, ([self.style_predictor._shapes] if self.style_predictor is not None
+                                                       else []) + [self._shapes], masks)]
+        return [x for group in reversed(named) for x in group]       # the transfer network's come first in the bucket
+
     def _checkpoint_tensors(self):
         from .tf_checkpoint import SLOT_MARK, VAR_SUFFIX, parts_tensors
         out = parts_tensors(self._checkpoint_parts())
         if self._handle is None:
+            return out
+        o = self.optimizer
+        if isinstance(o, AdamW):
+            for slot, values in zip("mv", o.slots()):
+                for (path, shape), value in zip(self._adamw_paths(), values):
+                    out[f"{path}{SLOT_MARK}optimizer/{slot}{VAR_SUFFIX}"] = value.cpu().numpy().reshape(shape)
+            out["optimizer/iter" + VAR_SUFFIX] = np.array(o.iterations, np.int64)
+            for name in _ADAMW_HYPER:
+                out[f"optimizer/{name}{VAR_SUFFIX}"] = np.array(getattr(o, name), np.float32)
             return out
         for part, mask, get, _ in self._slot_groups():
             for path, slot, trainable in zip(part.tree.paths(part.prefix), get(), mask):
@@ -344,6 +403,8 @@ class StyleTransferTrainingModel:
     def _restore_tensors(self, tensors):
         from .tf_checkpoint import SLOT_MARK, VAR_SUFFIX, restore_parts
         used, slot_sets = [], []
+        if self._handle is not None and isinstance(self.optimizer, AdamW):
+            return self._restore_adamw(tensors)
         if self._handle is not None:
             for part, mask, get, set_ in self._slot_groups():
                 keys = [f"{p}{SLOT_MARK}optimizer/rms{VAR_SUFFIX}" if t else None
@@ -367,6 +428,28 @@ class StyleTransferTrainingModel:
             for name in ("learning_rate", "rho"):
                 if f"optimizer/{name}{VAR_SUFFIX}" in tensors:
                     setattr(self.optimizer, name, float(tensors[f"optimizer/{name}{VAR_SUFFIX}"]))
+        return status
+
+    def _restore_adamw(self, tensors):
+        """Restore with an AdamW compiled: the weights and, where the checkpoint holds an AdamW's moments for every
+        variable, these, the step count and the hyperparameters."""
+        from .tf_checkpoint import SLOT_MARK, VAR_SUFFIX, restore_parts
+        o, paths = self.optimizer, self._adamw_paths()
+        keys = {slot: [f"{p}{SLOT_MARK}optimizer/{slot}{VAR_SUFFIX}" for p, _ in paths] for slot in "mv"}
+        hyper = {n: f"optimizer/{n}{VAR_SUFFIX}" for n in ("iter",) + _ADAMW_HYPER}
+        have = all(k in tensors for ks in keys.values() for k in ks)
+        used = [k for ks in keys.values() for k in ks] + [k for k in hyper.values() if k in tensors] if have else []
+        status = restore_parts(self._checkpoint_parts(), tensors, extra_keys=used)   # validates, then sets weights
+        if have:
+            m, v = ([torch.from_numpy(np.array(tensors[k], np.float32)) for k in keys[slot]] for slot in "mv")
+            o.set_slots(m, v)
+            if hyper["iter"] in tensors:
+                o.iterations = self.iterations = int(tensors[hyper["iter"]])
+                if self.style_predictor is not None:
+                    self.style_predictor.iterations = self.iterations
+            for n in _ADAMW_HYPER:
+                if hyper[n] in tensors:     # a float32 variable: its shortest decimal is the number that was set
+                    setattr(o, n, float(str(np.float32(tensors[hyper[n]]))))
         return status
 
     def load_weights(self, filepath):
@@ -467,11 +550,25 @@ class StyleTransferTrainingModel:
 
     def apply_gradients(self, grad: torch.Tensor):
         self._require_trainer()
-        self._version += 1
         o = self.optimizer
+        if isinstance(o, AdamW):
+            raise ValueError("AdamW steps the transfer network and the style predictor together, from the gradient "
+                             "bucket: use train_step")
+        self._version += 1
         _lib.check(_lib.load().rst_trainer_apply_gradients(self._handle, _lib.dev_ptr(grad), o.learning_rate, o.rho,
                                                            o.epsilon, _lib.stream_ptr()))
         self.iterations += 1
+
+    def _apply_adamw(self):
+        """One AdamW step of every trainable weight of both networks from the bucket, then the transfer network's
+        kernel images follow its weights (the predictor's kernels read theirs in place)."""
+        self.optimizer.apply_gradients(self._grad_bucket)
+        _lib.check(_lib.load().rst_trainer_weights_updated(self._handle, _lib.stream_ptr()))
+        self._version += 1
+        self.iterations += 1
+        if self.style_predictor is not None:
+            self.style_predictor._version += 1
+            self.style_predictor.iterations += 1
 
     def _world(self) -> int:
         dist = torch.distributed
@@ -583,8 +680,11 @@ class StyleTransferTrainingModel:
         if pr is not None:
             self._predictor_backward(pr, gsp)
         self.exchange()                       # one collective: gradients + BN moving statistics
-        self.apply_gradients(grad)
-        if pr is not None:
+        if isinstance(self.optimizer, AdamW):
+            self._apply_adamw()
+        else:
+            self.apply_gradients(grad)
+        if pr is not None and not isinstance(self.optimizer, AdamW):
             o = self.optimizer
             pr.apply_gradients(self._pgrad, o.learning_rate, o.rho, o.epsilon)
         self.style_losses = {n: losses[:, i] for i, n in enumerate(LOSS_NAMES)}
@@ -721,7 +821,7 @@ def make_style_transfer_training_model(style_predictor_factory_func: Optional[Ca
                                        style_transfer_factory_func: Callable,
                                        style_loss_func_factory_func: Callable,
                                        name="StyleTransferTrainingModel", max_batch: int = 4,
-                                       optimizer: Optional[RMSprop] = None, process_group=None,
+                                       optimizer=None, process_group=None,
                                        precision: str = "winograd_bf16x6"):
     """styleTransferTrainingModel.py:39-70 on librst.
 
@@ -752,5 +852,5 @@ def make_style_transfer_training_model(style_predictor_factory_func: Optional[Ca
     return StyleTransferModels(training, loss)
 
 
-__all__ = ['allreduce_gradients', 'RMSprop', 'StyleTransferTrainingModel', 'StyleTransferModels', 'make_style_transfer_training_model',
+__all__ = ['allreduce_gradients', 'RMSprop', 'AdamW', 'StyleTransferTrainingModel', 'StyleTransferModels', 'make_style_transfer_training_model',
            'make_style_loss_function', 'make_style_transfer_inference_model']

@@ -1,0 +1,483 @@
+"""The AdamW step on the GPU against its formula in float64.
+
+Tolerances, e = 2^-24. 32-bit states: m = fma(b1, m, c1 g) with rounded b1, c1 and (clipped) g: 4 e of the sum of the
+terms' sizes covers it; v has g twice more: 6 e. q = m / bc1 / (sqrt(v / bc2) + eps): its numerator carries m's error and
+2 e, its denominator half of v's error and 3 e, the division e: |dq| <= dm / (bc1 den) + 10 e |q|. p -= lr (q + wd p):
+lr (dq + 3 e (|q| + |wd p|)) and the last rounding, e |p|. 8-bit states: scales and codes are formed in 64 bits and have
+to be equal; m and v enter q rounded to f32 (2 e)."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+E = 2.0 ** -24
+LR, WD, B1, B2, EPS = 1e-2, 0.1, 0.9, 0.999, 1e-7
+SIZES = [[1], [127], [128], [129], [4096], [4097, 3, 1, 640], [5, 12289, 2, 2, 255, 33]]
+
+
+@pytest.fixture(autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.fail("needs a GPU")
+
+
+def _adamw(**kw):
+    from realtime_style_transfer_amd.optimizers import AdamW
+    return AdamW(**{**dict(learning_rate=LR, weight_decay=WD, beta_1=B1, beta_2=B2, epsilon=EPS), **kw})
+
+
+def _make(sizes, seed=0, gap=0):
+    """Variables with odd starts inside one buffer, their gradients' bucket, which of them decay."""
+    rng = np.random.default_rng(seed)
+    n = sum(sizes)
+    flat = torch.from_numpy(rng.standard_normal(n + 1).astype(np.float32)).cuda()[1:]
+    grad = torch.from_numpy((rng.standard_normal(n) * np.exp(rng.standard_normal(n))).astype(np.float32)).cuda()
+    return list(flat.split(sizes)), grad, [k % 2 == 0 for k in range(len(sizes))]
+
+
+def _mix(x):
+    x = x.astype(np.uint32)
+    with np.errstate(over='ignore'):
+        x = (x ^ (x >> np.uint32(16))) * np.uint32(0x7FEB352D)
+        x = (x ^ (x >> np.uint32(15))) * np.uint32(0x846CA68B)
+    return x ^ (x >> np.uint32(16))
+
+
+def _spacing(y):
+    return np.ldexp(1.0, np.maximum(np.frexp(np.maximum(np.abs(y), 1e-300))[1] - 1, -6) - 3)
+
+
+class Reference:
+    """The documented step in float64 on the host, states as the optimizer holds them."""
+
+    def __init__(self, opt, variables, decay):
+        self.sizes = [v.numel() for v in variables]
+        self.bits, self.seed, self.clip = opt.state_bits, opt.seed, opt.global_clipnorm
+        self.decay = np.concatenate([np.full(n, float(d)) for n, d in zip(self.sizes, decay)])
+        at = np.cumsum([0] + [-(-n // 128) * 128 for n in self.sizes])
+        self.place = np.concatenate([a + np.arange(n) for a, n in zip(at, self.sizes)])
+        self.padded = int(at[-1])
+
+    def read(self, opt, variables):
+        f = lambda t: t.detach().float().cpu().numpy().astype(np.float64)  # noqa: E731
+        s = {"p": np.concatenate([f(v).reshape(-1) for v in variables]), "m": f(opt.m), "v": f(opt.v),
+             "t": opt.iterations}
+        if self.bits == 8:
+            s["ms"], s["vs"] = f(opt.m_scale), f(opt.v_scale)
+        return s
+
+    def step(self, s, g):
+        g = g.astype(np.float64)
+        norm = np.sqrt((g * g).sum())
+        c = min(1.0, self.clip / norm) if self.clip else 1.0
+        t = s["t"] + 1
+        if self.bits == 32:
+            m0, v0 = s["m"], s["v"]
+        else:
+            m0, v0 = ((s[k] * s[k + "s"][:, None]).reshape(-1)[self.place] for k in "mv")
+        g = c * g
+        m, v = B1 * m0 + (1 - B1) * g, B2 * v0 + (1 - B2) * g * g
+        den = np.sqrt(v / (1 - B2 ** t)) + EPS
+        q = m / (1 - B1 ** t) / den
+        p = s["p"] - LR * (q + WD * self.decay * s["p"])
+        size_m = B1 * np.abs(m0) + (1 - B1) * np.abs(g)
+        dm = 4 * E * size_m if self.bits == 32 else 2 * E * np.abs(m)
+        dq = dm / (1 - B1 ** t) / den + 10 * E * np.abs(q)
+        out = {"p": p, "m": m, "v": v, "t": t, "norm": norm, "dm": dm, "dv": 6 * E * v,
+               "dp": LR * (dq + 3 * E * (np.abs(q) + np.abs(WD * s["p"]))) + E * np.abs(p) + 1e-38}
+        if self.bits == 8:
+            full = np.zeros((2, self.padded))
+            full[0, self.place], full[1, self.place] = m, v
+            for k, x in zip("mv", full.reshape(2, -1, 128)):
+                scale = (np.abs(x).max(1) / 448).astype(np.float32).astype(np.float64)
+                y = np.divide(x, scale[:, None], where=scale[:, None] > 0, out=np.zeros_like(x))
+                y = y.astype(np.float32).astype(np.float64)
+                step = _spacing(y)
+                if k == "m":
+                    code = np.round(y / step) * step
+                else:
+                    with np.errstate(over='ignore'):
+                        key = _mix(np.array([self.seed + t * 0x9E3779B9 & 0xFFFFFFFF]))
+                        h = _mix(np.arange(self.padded // 2).astype(np.uint32) ^ key)
+                    u = np.stack([h & np.uint32(0xFFFF), h >> np.uint32(16)], 1).reshape(y.shape)
+                    code = np.floor(y / step + u / 65536.0) * step
+                    code = np.where((x > 0) & (scale[:, None] > 0), np.maximum(code, 2.0 ** -9), code)
+                out[k], out[k + "s"] = np.clip(code, -448, 448), scale
+        return out
+
+
+def _compare(want, got, bits):
+    def near(k, tol):
+        off = np.abs(got[k] - want[k]) - tol
+        assert (off <= 0).all(), (k, float(off.max()), int(off.argmax()))
+    near("p", want["dp"])
+    assert got["t"] == want["t"]
+    if bits == 32:
+        near("m", want["dm"])
+        near("v", want["dv"])
+    else:
+        for k in ("m", "v", "ms", "vs"):
+            assert np.array_equal(got[k], want[k]), (k, int((got[k] != want[k]).sum()))
+
+
+@pytest.mark.parametrize("clip", [None, 0.7])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_steps(sizes, bits, dtype, clip):
+    variables, _, decay = _make(sizes)
+    opt = _adamw(state_bits=bits, global_clipnorm=clip, seed=3)
+    opt.build(variables, decay=decay)
+    ref = Reference(opt, variables, decay)
+    for k in range(4):                                  # from zero states on, each step from the device's own state
+        grad = (_make(sizes, seed=20 + k)[1] * (0.1 if k == 2 else 1.0)).to(dtype)
+        want = ref.step(ref.read(opt, variables), grad.float().cpu().numpy())
+        opt.apply_gradients(grad)
+        _compare(want, ref.read(opt, variables), bits)
+        if clip:
+            assert abs(float(opt.global_norm) - want["norm"]) <= 2 * E * want["norm"]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("t", [10 ** 3, 10 ** 6, 2 ** 33])
+def test_late_steps(bits, t):
+    """Step counts far on: 1 - beta^t from expm1 in 64 bits, the count in 64."""
+    variables, grad, decay = _make([700, 9])
+    opt = _adamw(state_bits=bits)
+    opt.build(variables, decay=decay)
+    rng = np.random.default_rng(4)
+    opt.set_slots([torch.from_numpy(rng.standard_normal(n)) for n in (700, 9)],
+                  [torch.from_numpy(rng.random(n)) for n in (700, 9)])
+    opt.iterations = t
+    ref = Reference(opt, variables, decay)
+    want = ref.step(ref.read(opt, variables), grad.cpu().numpy())
+    opt.apply_gradients(grad)
+    _compare(want, ref.read(opt, variables), bits)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_many_variables_as_a_bucket_and_as_a_list(bits):
+    """600 variables (more pointers than one launch carries): the same bits either way, and from separate tensors."""
+    rng = np.random.default_rng(5)
+    sizes = [int(n) for n in rng.integers(1, 300, 600)]
+    variables, grad, decay = _make(sizes)
+    copies = [v.clone() for v in variables]
+    a, b = _adamw(state_bits=bits, global_clipnorm=1.0), _adamw(state_bits=bits, global_clipnorm=1.0)
+    a.build(variables, decay=decay)
+    b.build(copies, decay=decay)
+    ref = Reference(a, variables, decay)
+    for k in range(3):
+        want = ref.step(ref.read(a, variables), grad.cpu().numpy())
+        a.apply_gradients(grad)
+        b.apply_gradients([g.clone() for g in grad.split(sizes)])
+        _compare(want, ref.read(a, variables), bits)
+        assert all(torch.equal(p, q) for p, q in zip(variables, copies))
+    assert torch.equal(a.m.view(torch.uint8), b.m.view(torch.uint8))
+    assert torch.equal(a.v.view(torch.uint8), b.v.view(torch.uint8))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("bad", [float('nan'), float('inf')])
+def test_a_clipped_step_with_a_bad_gradient_changes_nothing(bits, bad):
+    variables, grad, decay = _make([300, 5000])
+    opt = _adamw(state_bits=bits, global_clipnorm=1.0)
+    opt.build(variables, decay=decay)
+    opt.apply_gradients(grad)
+    before = [t.clone() for t in (*variables, opt.m.view(torch.uint8), opt.v.view(torch.uint8))]
+    worse = grad.clone()
+    worse[4321] = bad
+    opt.apply_gradients(worse)
+    assert not torch.isfinite(opt.global_norm)
+    assert all(torch.equal(p, q) for p, q in zip(before, (*variables, opt.m.view(torch.uint8), opt.v.view(torch.uint8))))
+    assert opt.iterations == 1
+    opt.apply_gradients(grad)                            # and the next one goes on
+    assert opt.iterations == 2 and torch.isfinite(opt.global_norm)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_zero_gradients_and_decay_alone(bits):
+    variables, grad, decay = _make([640, 130])
+    opt = _adamw(state_bits=bits, global_clipnorm=1.0)
+    opt.build(variables, decay=decay)
+    before = [v.clone() for v in variables]
+    opt.apply_gradients(torch.zeros_like(grad))
+    assert torch.equal(variables[1], before[1])          # no decay: untouched, no 0 / 0
+    off = (variables[0].double() - before[0].double() * (1 - LR * WD)).abs()
+    assert bool((off <= 3 * E * before[0].abs()).all())
+    assert not opt.m.float().any() and not opt.v.float().any() and float(opt.global_norm) == 0.0
+
+
+def test_second_moments_of_8_bits_follow_the_mean():
+    """The random rounding: after 1500 steps of gradients of constant size the mean of v over many elements is the
+    formula's g^2 (1 - b2^t) to 2 %; rounded to nearest it would stay near its first few steps' values (about
+    16 of 1000 ways up). Noise: a step's rounding has a variance of about 1e-3 v^2 / 12, kept for 1 / (2 (1 - b2))
+    steps: 0.2 of v, over 32768 elements 0.1 %; each block's largest element alone (1 of 128) is not rounded."""
+    n, g = 32768, 0.25
+    p = torch.zeros(n, device='cuda')
+    opt = _adamw(state_bits=8, weight_decay=0.0)
+    opt.build([p])
+    rng = torch.Generator().manual_seed(0)
+    sign = [(torch.randint(0, 2, (n,), generator=rng).float() * 2 - 1).cuda() * g for _ in range(8)]
+    size = torch.where(torch.arange(n, device='cuda') % 128 == 0, 4.0, 1.0)     # the block's largest sets the scale
+    for k in range(1500):
+        opt.apply_gradients(sign[k % 8] * size)
+    v = opt.slots()[1][0]
+    want = g * g * (1 - B2 ** 1500)
+    got = float(v[size == 1.0].double().mean())
+    assert abs(got / want - 1) < 0.02, (got, want)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_steps_count_on(bits):
+    """Replays are steps of their own (bias corrections, random bits), with eager steps between them."""
+    variables, grad, decay = _make([1000, 77, 4500])
+    copies = [v.clone() for v in variables]
+    a, b = (_adamw(state_bits=bits, global_clipnorm=1.0) for _ in range(2))
+    a.build(variables, decay=decay)
+    b.build(copies, decay=decay)
+    parts = list(grad.split([1000, 77, 4500]))
+    a.apply_gradients(grad)
+    torch.cuda.synchronize()
+    bucket, tensors = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(bucket):
+        a.apply_gradients(grad)
+    with torch.cuda.graph(tensors):
+        a.apply_gradients(parts)
+    for g in (bucket, None, tensors, bucket, None, bucket, tensors):
+        g.replay() if g is not None else a.apply_gradients(grad)
+        torch.cuda.synchronize()
+    for _ in range(8):
+        b.apply_gradients(grad)
+    assert a.iterations == b.iterations == 8
+    assert all(torch.equal(p, q) for p, q in zip(variables, copies))
+    assert torch.equal(a.v.view(torch.uint8), b.v.view(torch.uint8))
+
+
+def test_two_optimizers_on_two_streams():
+    made = [_make([5000, 12, 900], seed=k) for k in (1, 2)]
+    want = []
+    for variables, grad, decay in made:
+        c = [v.clone() for v in variables]
+        opt = _adamw(state_bits=8, global_clipnorm=1.0)
+        opt.build(c, decay=decay)
+        for _ in range(5):
+            opt.apply_gradients(grad)
+        want.append(c)
+    opts = []
+    for variables, _, decay in made:
+        opts.append(_adamw(state_bits=8, global_clipnorm=1.0))
+        opts[-1].build(variables, decay=decay)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for opt, st, (_, grad, _) in zip(opts, streams, made):
+            with torch.cuda.stream(st):
+                opt.apply_gradients(grad)
+    torch.cuda.synchronize()
+    for c, (variables, _, _) in zip(want, made):
+        assert all(torch.equal(p, q) for p, q in zip(c, variables))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_slots_round_trip(bits):
+    sizes = [300, 7, 128]
+    variables, grad, decay = _make(sizes)
+    opt = _adamw(state_bits=bits)
+    opt.build(variables, decay=decay)
+    for _ in range(3):
+        opt.apply_gradients(grad)
+    m, v = opt.slots()
+    other = _adamw(state_bits=bits)
+    other.build([t.clone() for t in variables], decay=decay)
+    other.set_slots([t.view(-1, 1) for t in m], v)
+    m2, v2 = other.slots()
+    if bits == 32:
+        assert all(torch.equal(p, q) for p, q in zip(m + v, m2 + v2))
+    else:
+        # the same codes, with a scale that went through fl(fl(448 s) / 448): a slot, fl(code s), moves by 4 e at most
+        assert torch.equal(opt.m.view(torch.uint8), other.m.view(torch.uint8))
+        assert all(bool(((p - q).abs() <= 4 * E * p.abs()).all()) for p, q in zip(m, m2))
+        # a block's largest v may have been rounded down, which moves the new scale by a code's step
+        assert all(bool(((p - q).abs() <= 2.0 ** -4 * p + 1e-30).all()) for p, q in zip(v, v2))
+    with pytest.raises(ValueError):
+        other.set_slots(m[:2], v[:2])
+
+
+def test_refusals_on_the_device():
+    from realtime_style_transfer_amd import _lib as L
+    variables, grad, _ = _make([10, 20])
+    opt = _adamw()
+    with pytest.raises(ValueError):
+        opt.build([variables[0], variables[1].double()])
+    with pytest.raises(ValueError):
+        opt.build([variables[0], variables[1].view(4, 5).t()])
+    opt.build(variables)
+    with pytest.raises(ValueError, match="already has variables"):
+        opt.build(variables)
+    for bad in (grad[:-1], grad.double(), grad.cpu(), torch.cat([grad, grad])[::2], [grad[:10]], [grad[:10], None],
+                [grad[:10], grad[10:].bfloat16()], [grad[:10], grad[:10]]):
+        with pytest.raises(ValueError):
+            opt.apply_gradients(bad)
+    opt.beta_1 = 1.5
+    with pytest.raises(ValueError):
+        opt.apply_gradients(grad)
+    assert opt.iterations == 0
+    with pytest.raises(ValueError):
+        opt.iterations = -1
+    assert L.load().rst_adamw_num_blocks(opt._handle) == 2
+
+
+def test_trains_a_normalised_layer():
+    """Forward, gradients and step together, as a training loop runs them: three steps of the affine and the input of a
+    group norm against the same loop in float64 (autograd, the formula). Each step's loss is the same to 1e-5 of its
+    size, as 32-bit outputs with 64-bit statistics keep it; Adam's first steps divide by |g|, so that an element whose
+    gradient is lost in rounding may go either way: variables are compared where |g| is not below 1e-3 of its rms."""
+    from realtime_style_transfer_amd.styleTransfer import group_norm, group_norm_gradients
+    g = torch.Generator().manual_seed(1)
+    shape, G = (2, 12, 10, 32), 8
+    x, scale, bias = (torch.randn(shape, generator=g).cuda(), 1 + 0.1 * torch.randn(32, generator=g).cuda(),
+                      torch.randn(32, generator=g).cuda())
+    target = torch.randn(shape, generator=g).cuda()
+    ref = [t.double().clone() for t in (x, scale, bias)]
+    state = [(torch.zeros_like(t), torch.zeros_like(t)) for t in ref]
+    solid = [torch.ones_like(t, dtype=torch.bool) for t in ref]
+    bucket = torch.empty(x.numel() + 64, device='cuda')
+    opt = _adamw(global_clipnorm=5.0)
+    opt.build([x, scale, bias], decay=[False, True, False])
+    for t in range(1, 4):
+        y, mean, rstd = group_norm(x, scale, bias, G, activation="swish", return_statistics=True)
+        grads = group_norm_gradients(x, y - target, scale, bias, mean, rstd, G, activation="swish")
+        torch.cat([d.reshape(-1) for d in grads], out=bucket)
+        opt.apply_gradients(bucket)
+        leaves = [t_.clone().requires_grad_() for t_ in ref]
+        r = leaves[0].reshape(2, 120, G, 4)
+        z = ((r - r.mean((1, 3), keepdim=True)) * (r.var((1, 3), unbiased=False, keepdim=True) + 1e-5).rsqrt()) \
+            .reshape(shape) * leaves[1] + leaves[2]
+        loss = 0.5 * ((z * torch.sigmoid(z) - target) ** 2).sum()
+        loss.backward()
+        mine = 0.5 * float(((y.double() - target) ** 2).sum())
+        assert abs(mine - float(loss)) < 1e-5 * float(loss) + (t > 1) * 1e-4 * float(loss)
+        norm = torch.sqrt(sum((l.grad ** 2).sum() for l in leaves))
+        c = min(1.0, 5.0 / float(norm))
+        for k, leaf in enumerate(leaves):
+            m, v = state[k]
+            gk = c * leaf.grad
+            solid[k] &= gk.abs() > 1e-3 * gk.norm() / gk.numel() ** 0.5
+            m.mul_(B1).add_((1 - B1) * gk)
+            v.mul_(B2).add_((1 - B2) * gk * gk)
+            ref[k] = ref[k] - LR * (m / (1 - B1 ** t) / (torch.sqrt(v / (1 - B2 ** t)) + EPS) + (WD if k == 1 else 0) * ref[k])
+    for mine, want, at in zip((x, scale, bias), ref, solid):
+        assert float(at.float().mean()) > 0.9
+        assert float((mine.double() - want)[at].abs().max()) < 1e-2 * 3 * LR
+
+
+def _training_model(optimizer, seed=2):
+    from realtime_style_transfer_amd.stylePrediction import StylePredictionTrainer
+    from realtime_style_transfer_amd.plan import network_plan
+    from realtime_style_transfer_amd.styleTransferTrainingModel import StyleTransferTrainingModel
+    ins, outs, br, bf = (32, 64, 17), (32, 64, 3), 8, 8
+    P = network_plan(ins, outs, br, bf).num_style_params
+    pr = StylePredictionTrainer((32, 64, 3), "MOBILE_NET", P, max_batch=2)
+    return StyleTransferTrainingModel(ins, outs, br, bf, max_batch=2, seed=seed, style_predictor=pr,
+                                      optimizer=optimizer)
+
+
+def _batch(seed=0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.rand(*s, generator=g).cuda()  # noqa: E731
+    return ({'content': r(2, 32, 64, 17), 'style': r(2, 1, 32, 64, 3)},
+            {'content': r(2, 32, 64, 3), 'style': r(2, 1, 32, 64, 3)})
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_training_model_steps_both_networks(bits):
+    """compile(optimizer=AdamW): every trainable weight of the transfer network and the predictor takes the formula's
+    step from the gradient bucket (one norm over both), kernels alone decay, BN moving statistics are left to the
+    forward, and the transfer network's kernel images follow."""
+    opt = _adamw(learning_rate=LR, global_clipnorm=1.0, state_bits=bits)
+    tr = _training_model(None)
+    tr.compile(optimizer=opt)
+    pr = tr.style_predictor
+    from realtime_style_transfer_amd.stylePrediction import trainable_mask
+    mask = [not k for k in _moving(tr)] + list(trainable_mask(pr.spec))
+    before = tr.get_weights() + pr.get_weights()
+    x, y = _batch()
+    tr.train_step(x, y)
+    after = tr.get_weights() + pr.get_weights()
+    flat = tr._grad_bucket.double().cpu().numpy()
+    norm = np.sqrt((flat ** 2).sum())
+    c, o = min(1.0, 1.0 / norm), 0
+    assert abs(float(opt.global_norm) / norm - 1) < 1e-6
+    for w0, w1, train in zip(before, after, mask):
+        g = c * flat[o:o + w0.size].reshape(w0.shape)
+        o += w0.size
+        if not train:
+            assert not g.any()
+            continue
+        q = g / (np.abs(g) + EPS)           # the first step: m / bc1 = g, sqrt(v / bc2) = |g|
+        want = w0 - LR * (q + (WD if w0.ndim > 1 else 0.0) * w0.astype(np.float64))
+        tol = LR * 16 * E * (np.abs(q) + 1) + 2 * E * np.abs(want)
+        assert (np.abs(w1 - want) <= tol).all(), float((np.abs(w1 - want) - tol).max())
+    assert o == flat.size and opt.iterations == tr.iterations == pr.iterations == 1
+    # a model made anew from these weights gives the same losses: the kernels' images were re-packed
+    other = _training_model(_adamw())
+    other.set_weights(tr.get_weights())
+    pr2 = other.style_predictor
+    pr2.set_weights(pr.get_weights())
+    for m in (tr, other):
+        m.train_step(x, y)
+    assert torch.equal(tr.style_losses['loss'], other.style_losses['loss'])
+
+
+def _moving(tr):
+    out = []
+    for layer in tr.plan.layers:
+        out += [False, False] + ([False, False, True, True] if layer.norm == 'bn' else [])
+    return out
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_training_checkpoint_restores_the_moments(bits, tmp_path):
+    x, y = _batch()
+    a = _training_model(_adamw(state_bits=bits))
+    for _ in range(3):
+        a.train_step(x, y)
+    a.save_weights(str(tmp_path / "ck"))
+    a.optimizer.learning_rate = 5e-3
+    a.save_weights(str(tmp_path / "ck"))
+    b = _training_model(_adamw(state_bits=bits), seed=5)
+    b.load_weights(str(tmp_path / "ck")).assert_nontrivial_match()
+    assert b.iterations == b.optimizer.iterations == 3 and abs(b.optimizer.learning_rate - 5e-3) < 1e-9
+    for p, q in zip(a.optimizer.slots()[0], b.optimizer.slots()[0]):      # 4 e: test_slots_round_trip
+        assert torch.equal(p, q) if bits == 32 else bool(((p - q).abs() <= 4 * E * p.abs()).all())
+    for p, q in zip(a.optimizer.slots()[1], b.optimizer.slots()[1]):
+        assert torch.equal(p, q) if bits == 32 else bool(((p - q).abs() <= 2.0 ** -4 * p + 1e-30).all())
+    if bits == 32:
+        for m in (a, b):
+            m.train_step(x, y)
+        assert all(np.array_equal(p, q) for p, q in zip(a.get_weights(), b.get_weights()))
+    # the moments are no RMSprop state: restored into an RMSprop model they are reported unused
+    from realtime_style_transfer_amd.styleTransferTrainingModel import RMSprop
+    c = _training_model(RMSprop())
+    status = c.load_weights(str(tmp_path / "ck"))
+    with pytest.raises(AssertionError):
+        status.assert_consumed()
+
+
+def test_training_model_refusals():
+    tr = _training_model(_adamw())
+    with pytest.raises(ValueError, match="train_step"):
+        tr.apply_gradients(tr._grad)
+    with pytest.raises(ValueError, match="already has variables"):
+        _training_model(tr.optimizer)
+    with pytest.raises(TypeError):
+        tr.compile(optimizer=torch.optim.SGD([torch.zeros(1, requires_grad=True)], 0.1))
+    with pytest.raises(ValueError, match="optimizer_slots"):
+        tr.optimizer_slots()
+    opt = tr.optimizer
+    size = opt._bucket_size
+    del tr
+    import gc
+    gc.collect()
+    with pytest.raises(ValueError, match="no longer exists"):
+        opt.apply_gradients(torch.zeros(size, device='cuda'))
