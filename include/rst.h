@@ -156,11 +156,12 @@ int rst_instance_norm(const float* x, int batch, int hw, int channels, const flo
  * runs on 16-byte loads. y may be x. mean / rstd (B, groups) receive the statistics when not NULL.
  * backward: from dy, x and the forward's mean / rstd: dx (may be dy), dscale and dbias shaped as scale / bias (sums over
  * the batch where they are shared). The same inputs give the same bits (no atomics). batch or hw 0: RST_OK, nothing is
- * written but dscale = dbias = 0. workspace: rst_group_norm_workspace_size() bytes, aligned to 16, used by one call at a
- * time (calls on two streams, or two captured graphs that may replay together, need one each). */
+ * written but dscale = dbias = 0. workspace: rst_group_norm(_backward)_workspace_size() bytes (0: may be NULL), aligned to
+ * 16, used by one call at a time (calls on two streams, or two captured graphs that may replay together, need one each). */
 enum { RST_DTYPE_FLOAT32 = 0, RST_DTYPE_BFLOAT16 = 1 };
 enum { RST_ACT_LINEAR = 0, RST_ACT_RELU = 1, RST_ACT_SWISH = 2, RST_ACT_HARD_SWISH = 3 };
 size_t rst_group_norm_workspace_size(int batch, int hw, int channels, int groups);
+size_t rst_group_norm_backward_workspace_size(int batch, int hw, int channels, int groups);
 int rst_group_norm(const void* x, int dtype, int batch, int hw, int channels, int groups, const float* scale,
                    const float* bias, int per_image, float eps, int activation, void* y, float* mean, float* rstd,
                    void* workspace, void* stream);
@@ -349,13 +350,13 @@ int rst_predictor_trainer_set_moving_statistics(rst_predictor_trainer* t, const 
  *   state_bits 32: m, v f32, the variables' elements one after the other (no gaps).
  *   state_bits 8: m, v e4m3 codes in blocks of 128 elements of one variable, the variables' blocks one after the other
  *     (a variable's last block is filled with zeros), aligned to 8 bytes; m_scale, v_scale one f32 per block. A state
- *     is code * scale, scale = max / 448. m / scale rounds to nearest; v / scale rounds up or down at random with the
+ *     is code * scale, scale = max / 448 (0 where that would be below 2^-126). m / scale rounds to nearest; v / scale rounds up or down at random with the
  *     right mean (bits from a hash of the element, the step and `seed`), never from above zero to zero. The step uses
  *     the m and v before they are rounded.
  *   iterations: steps taken (t = iterations + 1), moved on by every step on the device: a captured step replays as the
  *     next one. Hyperparameters are captured by value.
  *   global_norm: receives |g| of each step that clips (may be NULL). If |g| is not finite that step changes nothing,
- *     iterations included. Without clipping a NaN or infinity spreads as the formula says (with 8 bits: to its block).
+ *     iterations included. Without clipping a NaN spreads as the formula says, with 8 bits an infinity to its block.
  * States start as zeros (iterations 0). One step of a handle at a time: not on two streams at once. */
 typedef struct rst_adamw_tensor {
     float* param;

@@ -25,7 +25,7 @@ EXPORTED_SYMBOLS = [
     "rst_create", "rst_create_ex", "rst_precision", "rst_destroy", "rst_num_style_params", "rst_num_weights_for_shape", "rst_forward",
     "rst_num_layers", "rst_layer_output_shape", "rst_copy_activation", "rst_gram_workspace_size", "rst_gram",
     "rst_instance_norm_workspace_size", "rst_instance_norm", "rst_style_param_map", "rst_last_error", "rst_version",
-    "rst_group_norm_workspace_size", "rst_group_norm", "rst_group_norm_backward",
+    "rst_group_norm_workspace_size", "rst_group_norm_backward_workspace_size", "rst_group_norm", "rst_group_norm_backward",
     "rst_adamw_create", "rst_adamw_destroy", "rst_adamw_num_blocks", "rst_adamw_step", "rst_adamw_step_tensors",
     "rst_trainer_weights", "rst_trainer_weights_updated", "rst_predictor_trainer_weights",
     "rst_profile_begin", "rst_profile_end", "rst_timeline_begin", "rst_timeline_read", "rst_timeline_end",
@@ -160,6 +160,8 @@ def load() -> ctypes.CDLL:
     lib.rst_style_param_map.restype = i
     lib.rst_group_norm_workspace_size.argtypes = [i, i, i, i]
     lib.rst_group_norm_workspace_size.restype = sz
+    lib.rst_group_norm_backward_workspace_size.argtypes = [i, i, i, i]
+    lib.rst_group_norm_backward_workspace_size.restype = sz
     lib.rst_group_norm.argtypes = [vp, i, i, i, i, i, vp, vp, i, fp, i, vp, vp, vp, vp, vp]
     lib.rst_group_norm.restype = i
     lib.rst_group_norm_backward.argtypes = [vp, vp, i, i, i, i, i, vp, vp, i, vp, vp, i, vp, vp, vp, vp, vp]
@@ -298,6 +300,12 @@ def check(code: int):
 def stream_ptr(stream=None) -> int:
     s = torch.cuda.current_stream() if stream is None else stream
     return int(s.cuda_stream)
+
+
+def device_stream(index: int) -> int:
+    """The current stream of device ``index`` (what torch's own generated code calls: stream_ptr takes 3 us of a short
+    operator's 10)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def as_device(x, device) -> torch.Tensor:

@@ -8,6 +8,8 @@ namespace rst {
 constexpr int ADAMW_BLOCK = 128;       // elements of one 8-bit state block (and its scale)
 constexpr int ADAMW_CHUNK = 4096;      // elements of one workgroup: a multiple of the block
 constexpr int ADAMW_MAX_PARTIALS = 1024;
+constexpr int ADAMW_TICKETS = 64;      // workgroups that share a counter
+constexpr int ADAMW_TICKET_STRIDE = 32;   // a cache line
 constexpr int ADAMW_PTRS = 256;        // gradient pointers that one launch carries to the device
 
 // A workgroup's share of one variable
@@ -34,7 +36,7 @@ struct AdamwArgs {
     float* v_scale;
     long long* iterations;
     float* global_norm;                // may be null without clipping
-    unsigned* ticket;
+    unsigned* tickets;                 // a root and one per ADAMW_TICKETS workgroups, ADAMW_TICKET_STRIDE apart
     const double* partials;            // sums of squares of the gradient
     int num_partials;                  // 0: no clipping
     double lr, decay, b1, b2, eps, clip;
@@ -48,6 +50,7 @@ struct AdamwPtrs {
 
 hipError_t adamw_set_pointers_launch(const AdamwPtrs& p, const void** dst, int n, hipStream_t st);
 hipError_t adamw_norm_launch(const AdamwArgs& a, double* partials, hipStream_t st);
-hipError_t adamw_step_launch(const AdamwArgs& a, int state_bits, hipStream_t st);
+// past: loads and stores past the caches
+hipError_t adamw_step_launch(const AdamwArgs& a, int state_bits, bool past, hipStream_t st);
 
 }  // namespace rst

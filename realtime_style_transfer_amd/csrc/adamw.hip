@@ -31,15 +31,36 @@ typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float widen(unsigned short v) { return __uint_as_float((unsigned)v << 16); }
 
-__device__ __forceinline__ f32x4 load_grad4(const void* g, long long i, int bf16) {
-    if (bf16) {
-        const u16x4 v = *(const u16x4_u*)((const unsigned short*)g + i);
+// (pointers out of a table are generic: say that they are global)
+template <typename T>
+using Global = T __attribute__((address_space(1)))*;
+
+// PAST: past the caches, for a step whose data does not stay in them
+template <bool PAST, typename T>
+__device__ __forceinline__ T load(const void* p, long long i) {
+    const Global<const T> g = (Global<const T>)((const char*)p + i);
+    if constexpr (PAST) return __builtin_nontemporal_load(g);
+    else return *g;
+}
+template <bool PAST, typename T>
+__device__ __forceinline__ void store(void* p, long long i, T v) {
+    const Global<T> g = (Global<T>)((char*)p + i);
+    if constexpr (PAST) __builtin_nontemporal_store(v, g);
+    else *g = v;
+}
+
+template <bool BF16, bool PAST>
+__device__ __forceinline__ f32x4 load_grad4(const void* g, long long i) {
+    if constexpr (BF16) {
+        const u16x4 v = load<PAST, u16x4_u>(g, 2 * i);
         return f32x4{widen(v.x), widen(v.y), widen(v.z), widen(v.w)};
     }
-    return *(const f32x4_u*)((const float*)g + i);
+    return load<PAST, f32x4_u>(g, 4 * i);
 }
-__device__ __forceinline__ float load_grad(const void* g, long long i, int bf16) {
-    return bf16 ? widen(((const unsigned short*)g)[i]) : ((const float*)g)[i];
+template <bool BF16>
+__device__ __forceinline__ float load_grad(const void* g, long long i) {
+    if constexpr (BF16) return widen(load<false, unsigned short>(g, 2 * i));
+    return load<false, float>(g, 4 * i);
 }
 
 // The chunk's gradient: a base and an element index
@@ -60,109 +81,161 @@ __global__ __launch_bounds__(ADAMW_PTRS) void set_pointers_kernel(AdamwPtrs p, c
 }
 
 // Sums of squares over the chunks blockIdx, blockIdx + grid, ...: one partial per workgroup, merged by the step
-__global__ __launch_bounds__(NT) void norm_kernel(AdamwArgs a, double* __restrict__ partials) {
+template <bool BF16>
+__global__ __launch_bounds__(NT) void norm_kernel(AdamwArgs a, double* partials) {
     __shared__ double red[4];
+    constexpr int R = ADAMW_CHUNK / (4 * NT);
     double s = 0.0;
     for (int k = blockIdx.x; k < a.num_chunks; k += gridDim.x) {
         const AdamwChunk c = a.chunks[k];
         long long at;
         const void* g = grad_of(a, c, at);
-        for (int i = threadIdx.x * 4; i < c.count; i += NT * 4) {
-            if (i + 4 <= c.count) {
-                const f32x4 v = load_grad4(g, at + i, a.grad_bf16);
-                s = fma((double)v.x, (double)v.x, fma((double)v.y, (double)v.y,
-                    fma((double)v.z, (double)v.z, fma((double)v.w, (double)v.w, s))));
-            } else {
-                for (int j = i; j < c.count; ++j) {
-                    const double v = load_grad(g, at + j, a.grad_bf16);
-                    s = fma(v, v, s);
-                }
-            }
+        const int i0 = threadIdx.x * 4;
+        const int vectors = c.count / 4, tail = vectors * 4 + threadIdx.x;
+        if (vectors > 0) {
+            f32x4 v[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) v[r] = load_grad4<BF16, false>(g, at + (i0 / 4 + r * NT < vectors ? i0 + r * 4 * NT : 0));
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (i0 / 4 + r * NT < vectors)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) s = fma((double)v[r][q], (double)v[r][q], s);
+        }
+        if (tail < c.count) {
+            const double v = load_grad<BF16>(g, at + tail);
+            s = fma(v, v, s);
         }
     }
     s = block_sum(s, red);
     if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
-// What the whole step shares: the clipping factor, the step number and its corrections; false: nothing to do, the
-// gradient's norm is not finite
+// Whether this is the last of n to count; the counter is then zero again for the next step
+__device__ __forceinline__ bool last_of(unsigned* ticket, unsigned n) {
+    const bool last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+    if (last) *ticket = 0;
+    return last;
+}
+
+// What the whole step shares: the clipping factor, the step number and its corrections; `last`: this workgroup is the
+// last one to have read the step count and moves it on at its end. False: nothing to do, the gradient's norm is not
+// finite. Called with the chunk's loads under way.
 struct StepScalars {
-    double coef, inv_bc1, inv_bc2;
+    double coef;
+    float inv_bc1, inv_bc2;
     long long t;
+    bool last;
 };
 __device__ __forceinline__ bool step_scalars(const AdamwArgs& a, StepScalars& s, double* red) {
     s.t = *a.iterations + 1;
+    // 1 - beta^t: f32 is enough for the relative size of a step (the argument in 64 bits: t may be large)
+    s.inv_bc1 = -1.f / expm1f((float)((double)s.t * a.log_b1));
+    s.inv_bc2 = -1.f / expm1f((float)((double)s.t * a.log_b2));
     s.coef = 1.0;
     if (a.num_partials > 0) {
         double q = 0.0;
-        for (int i = threadIdx.x; i < a.num_partials; i += NT) q += a.partials[i];
+#pragma unroll
+        for (int i = 0; i < ADAMW_MAX_PARTIALS / NT; ++i) {
+            const int k = i * NT + threadIdx.x;
+            const double v = a.partials[min(k, a.num_partials - 1)];
+            q += k < a.num_partials ? v : 0.0;
+        }
         const double norm = sqrt(block_sum(q, red));
         if (blockIdx.x == 0 && threadIdx.x == 0 && a.global_norm != nullptr) *a.global_norm = (float)norm;
         if (!(norm < __builtin_inf())) return false;
         if (norm > a.clip) s.coef = a.clip / norm;
     }
-    s.inv_bc1 = -1.0 / expm1((double)s.t * a.log_b1);
-    s.inv_bc2 = -1.0 / expm1((double)s.t * a.log_b2);
+    __syncthreads();             // every wave has read the count
+    s.last = threadIdx.x == 0 && last_of(a.tickets + (1 + blockIdx.x / ADAMW_TICKETS) * ADAMW_TICKET_STRIDE,
+                                         min((unsigned)ADAMW_TICKETS, (unsigned)a.num_chunks - blockIdx.x / ADAMW_TICKETS * ADAMW_TICKETS));
     return true;
 }
 
-// The last workgroup moves the step count on: every other one has read it
-__device__ __forceinline__ void step_done(const AdamwArgs& a, long long t) {
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const unsigned n = __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (n == (unsigned)a.num_chunks - 1) {
-            *a.ticket = 0;
-            *a.iterations = t;
-        }
-    }
+// Workgroups count in groups of 64, and the last of each group at the root: with 872 workgroups at one address the step
+// took 18.2 us (8-bit states 21.4), like this 13.9 (16.0)
+__device__ __forceinline__ void step_done(const AdamwArgs& a, const StepScalars& s) {
+    if (s.last && last_of(a.tickets, (a.num_chunks + ADAMW_TICKETS - 1) / ADAMW_TICKETS)) *a.iterations = s.t;
+}
+
+// m / bc1 / (sqrt(v / bc2) + eps) through the hardware's root and reciprocal, one unit in the last place each
+__device__ __forceinline__ float quotient(float m, float v, float inv_bc1, float inv_bc2, float eps) {
+    return m * inv_bc1 * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v * inv_bc2) + eps);
 }
 
 struct Scalars32 {
-    float b1, c1, b2, c2, inv_bc1, inv_bc2, eps, lr, decay;
+    float b1, c1, b2, c2, inv_bc1, inv_bc2, eps, lr, decay, coef;
 };
 
 __device__ __forceinline__ void adamw_element(float g, float& p, float& m, float& v, const Scalars32& s) {
+    g *= s.coef;
     m = fmaf(s.b1, m, s.c1 * g);
     v = fmaf(s.b2, v, s.c2 * (g * g));
-    const float q = (m * s.inv_bc1) / (sqrtf(v * s.inv_bc2) + s.eps);
-    p = fmaf(-s.lr, fmaf(s.decay, p, q), p);
+    p = fmaf(-s.lr, fmaf(s.decay, p, quotient(m, v, s.inv_bc1, s.inv_bc2, s.eps)), p);
 }
 
+template <bool BF16, bool PAST>
 __global__ __launch_bounds__(NT) void adamw32_kernel(AdamwArgs a) {
     __shared__ double red[4];
+    constexpr int R = ADAMW_CHUNK / (4 * NT);
     const AdamwChunk c = a.chunks[blockIdx.x];
+    long long at;
+    const void* g = grad_of(a, c, at);
+    float* p = c.param;
+    float* m = (float*)a.m + c.state_at;
+    float* v = (float*)a.v + c.state_at;
+    const int i0 = threadIdx.x * 4;
+    const bool full = c.count == ADAMW_CHUNK;
+    // whole vectors first, then one element for each of the first count % 4 threads. Loads are unconditional (a guarded
+    // one would be waited for by itself): where there is no vector, the variable's first elements again
+    const int vectors = c.count / 4, rest = c.count % 4, tail = vectors * 4 + threadIdx.x;
+    f32x4 gv[R], pv[R], mv[R], vv[R];
+    float gt = 0.f, pt = 0.f, mt = 0.f, vt = 0.f;
+    if (vectors > 0) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = full || i0 / 4 + r * NT < vectors ? i0 + r * 4 * NT : 0;
+            gv[r] = load_grad4<BF16, PAST>(g, at + i);
+            pv[r] = load<PAST, f32x4_u>(p, 4ll * i);
+            mv[r] = load<PAST, f32x4_u>(m, 4ll * i);
+            vv[r] = load<PAST, f32x4_u>(v, 4ll * i);
+        }
+    }
+    if ((int)threadIdx.x < rest) {
+        gt = load_grad<BF16>(g, at + tail);
+        pt = load<false, float>(p, 4ll * tail);
+        mt = load<false, float>(m, 4ll * tail);
+        vt = load<false, float>(v, 4ll * tail);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     StepScalars st;
     const bool go = step_scalars(a, st, red);
     if (!go) return;
-    const Scalars32 s{(float)a.b1, (float)(1.0 - a.b1), (float)a.b2, (float)(1.0 - a.b2), (float)st.inv_bc1,
-                      (float)st.inv_bc2, (float)a.eps, (float)a.lr, c.decay ? (float)a.decay : 0.f};
-    const float coef = (float)st.coef;
-    long long at;
-    const void* g = grad_of(a, c, at);
-    float* __restrict__ p = c.param;
-    float* __restrict__ m = (float*)a.m + c.state_at;
-    float* __restrict__ v = (float*)a.v + c.state_at;
-    for (int i = threadIdx.x * 4; i < c.count; i += NT * 4) {
-        if (i + 4 <= c.count) {
-            const f32x4 gv = load_grad4(g, at + i, a.grad_bf16);
-            f32x4 pv = *(const f32x4_u*)(p + i), mv = *(const f32x4_u*)(m + i), vv = *(const f32x4_u*)(v + i);
+    const Scalars32 s{(float)a.b1, (float)(1.0 - a.b1), (float)a.b2, (float)(1.0 - a.b2), st.inv_bc1, st.inv_bc2,
+                      (float)a.eps, (float)a.lr, c.decay ? (float)a.decay : 0.f, (float)st.coef};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float pk = pv[k], mk = mv[k], vk = vv[k];
-                adamw_element(gv[k] * coef, pk, mk, vk, s);
-                pv[k] = pk;
-                mv[k] = mk;
-                vv[k] = vk;
-            }
-            *(f32x4_u*)(p + i) = pv;
-            *(f32x4_u*)(m + i) = mv;
-            *(f32x4_u*)(v + i) = vv;
-        } else {
-            for (int j = i; j < c.count; ++j) adamw_element(load_grad(g, at + j, a.grad_bf16) * coef, p[j], m[j], v[j], s);
+    for (int r = 0; r < R; ++r) {
+        if (!(full || i0 / 4 + r * NT < vectors)) break;
+        const int i = i0 + r * 4 * NT;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float pk = pv[r][k], mk = mv[r][k], vk = vv[r][k];
+            adamw_element(gv[r][k], pk, mk, vk, s);
+            pv[r][k] = pk;
+            mv[r][k] = mk;
+            vv[r][k] = vk;
         }
+        store<PAST, f32x4_u>(p, 4ll * i, pv[r]);
+        store<PAST, f32x4_u>(m, 4ll * i, mv[r]);
+        store<PAST, f32x4_u>(v, 4ll * i, vv[r]);
     }
-    step_done(a, st.t);
+    if ((int)threadIdx.x < rest) {
+        adamw_element(gt, pt, mt, vt, s);
+        store<false, float>(p, 4ll * tail, pt);
+        store<false, float>(m, 4ll * tail, mt);
+        store<false, float>(v, 4ll * tail, vt);
+    }
+    step_done(a, st);
 }
 
 // ---- 8-bit states --------------------------------------------------------------------------------------------------
@@ -174,135 +247,176 @@ __device__ __forceinline__ unsigned mix(unsigned x) {
     return x ^ (x >> 16);
 }
 
-// y in [0, 448] to an e4m3 code, up with the probability of its place between two codes (u: 16 random bits)
+// y in [0, 448] to an e4m3 code, up with the probability of its place between two codes (u: 16 random bits). An f32 has
+// 20 bits below e4m3's three; below 2^-6 codes are 2^-9 apart. A NaN gives the NaN code.
 __device__ __forceinline__ unsigned round_random(float y, unsigned u) {
-    const unsigned r = u << 4;       // an f32 has 20 bits below e4m3's three
-    unsigned code;
-    if (y < 0.015625f)               // below 2^-6 codes are 2^-9 apart
-        code = ((unsigned)(y * 536870912.f) + r) >> 20;
-    else
-        code = ((__float_as_uint(y) + r) >> 20) - ((127 - 7) << 3);
-    return code > 0x7Eu ? 0x7Eu : code;
+    const unsigned bits = y < 0.015625f ? (unsigned)(y * 536870912.f) : __float_as_uint(y) - ((127u - 7u) << 23);
+    return min((bits + (u << 4)) >> 20, 0x7Fu);
 }
 
-__device__ __forceinline__ double max16(double v) {     // over the 16 lanes of a block
-    for (int o = 8; o > 0; o >>= 1) {
-        const double w = __shfl_xor(v, o);
-        v = (w > v || w != w) ? w : v;                  // a NaN wins
+// Over the 16 lanes of a block, by permutations within the row of lanes
+template <int CTRL>
+__device__ __forceinline__ double max_dpp(double v) {
+    const long long b = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)(b & 0xFFFFFFFFll), CTRL, 0xF, 0xF, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_fmax(v, __longlong_as_double(((long long)hi << 32) | (unsigned)lo));
+}
+__device__ __forceinline__ double max16(double v) {
+    return max_dpp<0x140>(max_dpp<0x141>(max_dpp<0x4E>(max_dpp<0xB1>(v))));   // lanes xor 1, xor 2, the half mirrored, the row
+}
+
+// A block's scale from its largest value. One that would be subnormal is 0: the block counts as zeros
+__device__ __forceinline__ float scale_of(double largest) {
+    const float s = (float)(largest * (1.0 / 448.0));
+    return s < 1.17549435e-38f ? 0.f : s;
+}
+// 1 / s in 64 bits (one Newton step on the hardware's reciprocal: about one unit in the last place), 0 of 0
+__device__ __forceinline__ double inverse(float s) {
+    const double d = (double)s;
+    const double r = __builtin_amdgcn_rcp(d);
+    return s == 0.f ? 0.0 : fma(fma(-d, r, 1.0), r, r);
+}
+
+// One lane's eight elements: gradient, variable, codes, the block's scales
+struct Eight {
+    float g[8], p[8];
+    u32x2 m, v;
+    float ms, vs;
+};
+
+// Loads eight elements from element i of the chunk on; n of them are the variable's (the others: zeros)
+template <bool BF16, bool PAST, bool FULL>
+__device__ __forceinline__ void load8(Eight& e, const AdamwArgs& a, const AdamwChunk& c, const void* g, long long at, int i, int n) {
+    if constexpr (FULL) {
+#pragma unroll
+        for (int k = 0; k < 8; k += 4) {
+            const f32x4 x = load_grad4<BF16, PAST>(g, at + i + k), y = load<PAST, f32x4_u>(c.param, 4ll * (i + k));
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                e.g[k + q] = x[q];
+                e.p[k + q] = y[q];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {        // (unconditional loads, of the variable's last element beyond it)
+            const int q = min(i + k, c.count - 1);
+            e.g[k] = load_grad<BF16>(g, at + q);
+            e.p[k] = load<false, float>(c.param, 4ll * q);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k >= n) e.g[k] = 0.f;
     }
-    return v;
+    e.m = load<PAST, u32x2>(a.m, c.state_at + i);
+    e.v = load<PAST, u32x2>(a.v, c.state_at + i);
+    const long long block = (c.state_at + i) / ADAMW_BLOCK;
+    e.ms = a.m_scale[block];
+    e.vs = a.v_scale[block];
 }
 
-// Eight elements per lane, 16 lanes per block
-__global__ __launch_bounds__(NT) void adamw8_kernel(AdamwArgs a) {
+struct Scalars8 {
+    double b1, c1, b2, c2;        // c1, c2 with the clipping factor and its square
+    float inv_bc1, inv_bc2, eps, lr, decay;
+    unsigned key;
+};
+
+// Their step: 16 lanes are a block
+template <bool PAST, bool FULL>
+__device__ __forceinline__ void step8(Eight& e, const AdamwArgs& a, const AdamwChunk& c, int i, int n, const Scalars8& s) {
+    float mf[8], vf[8];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        mf[4 * k] = __builtin_amdgcn_cvt_f32_fp8(e.m[k], 0);
+        mf[4 * k + 1] = __builtin_amdgcn_cvt_f32_fp8(e.m[k], 1);
+        mf[4 * k + 2] = __builtin_amdgcn_cvt_f32_fp8(e.m[k], 2);
+        mf[4 * k + 3] = __builtin_amdgcn_cvt_f32_fp8(e.m[k], 3);
+        vf[4 * k] = __builtin_amdgcn_cvt_f32_fp8(e.v[k], 0);
+        vf[4 * k + 1] = __builtin_amdgcn_cvt_f32_fp8(e.v[k], 1);
+        vf[4 * k + 2] = __builtin_amdgcn_cvt_f32_fp8(e.v[k], 2);
+        vf[4 * k + 3] = __builtin_amdgcn_cvt_f32_fp8(e.v[k], 3);
+    }
+    const double ms = s.b1 * (double)e.ms, vs = s.b2 * (double)e.vs;
+    double m[8], v[8], mm = 0.0, vm = 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const double gd = (double)e.g[k];
+        m[k] = fma(ms, (double)mf[k], s.c1 * gd);
+        v[k] = fma(vs, (double)vf[k], s.c2 * (gd * gd));
+        mm = __builtin_fmax(mm, fabs(m[k]));      // (leaves a NaN out: it stays with its element)
+        vm = __builtin_fmax(vm, v[k]);
+        const float q = quotient((float)m[k], (float)v[k], s.inv_bc1, s.inv_bc2, s.eps);
+        e.p[k] = fmaf(-s.lr, fmaf(s.decay, e.p[k], q), e.p[k]);
+    }
+    if constexpr (FULL) {
+#pragma unroll
+        for (int k = 0; k < 8; k += 4)
+            store<PAST, f32x4_u>(c.param, 4ll * (i + k), f32x4{e.p[k], e.p[k + 1], e.p[k + 2], e.p[k + 3]});
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < n) c.param[i + k] = e.p[k];
+    }
+    const float new_ms = scale_of(max16(mm)), new_vs = scale_of(max16(vm));
+    const double im = inverse(new_ms), iv = inverse(new_vs);
+    const unsigned least = new_vs > 0.f ? 1u : 0u, pair = (unsigned)((unsigned long long)(c.state_at + i) >> 1);
+    u32x2 mo, vo;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        // (|m / s| is at most 448 and a rounding: no clamp)
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32((float)(m[4 * k] * im), (float)(m[4 * k + 1] * im), 0, false);
+        w = __builtin_amdgcn_cvt_pk_fp8_f32((float)(m[4 * k + 2] * im), (float)(m[4 * k + 3] * im), w, true);
+        mo[k] = (unsigned)w;
+        unsigned b = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const unsigned h = mix((pair + 2 * k + q / 2) ^ s.key);
+            const double x = v[4 * k + q];
+            b |= max(round_random((float)(x * iv), (q & 1) ? h >> 16 : h & 0xFFFFu), x > 0.0 ? least : 0u) << (8 * q);
+        }
+        vo[k] = b;
+    }
+    store<PAST, u32x2>(a.m, c.state_at + i, mo);
+    store<PAST, u32x2>(a.v, c.state_at + i, vo);
+    if ((threadIdx.x & 15) == 0) {
+        const long long block = (c.state_at + i) / ADAMW_BLOCK;
+        a.m_scale[block] = new_ms;
+        a.v_scale[block] = new_vs;
+    }
+}
+
+// Eight elements per lane and round: a chunk is two rounds
+template <bool BF16, bool PAST>
+__global__ __launch_bounds__(NT, 3) void adamw8_kernel(AdamwArgs a) {
     __shared__ double red[4];
+    constexpr int R = ADAMW_CHUNK / (8 * NT);
     const AdamwChunk c = a.chunks[blockIdx.x];
+    long long at;
+    const void* g = grad_of(a, c, at);
+    const int i0 = threadIdx.x * 8;
+    const int filled = (c.count + ADAMW_BLOCK - 1) / ADAMW_BLOCK * ADAMW_BLOCK;      // with the last block's zeros
+    Eight e[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = i0 + r * 8 * NT;
+        if (c.count == ADAMW_CHUNK) load8<BF16, PAST, true>(e[r], a, c, g, at, i, 8);
+        else if (i < filled) load8<BF16, PAST, false>(e[r], a, c, g, at, i, c.count - i);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     StepScalars st;
     const bool go = step_scalars(a, st, red);
     if (!go) return;
-    const unsigned key = mix(a.seed + (unsigned)st.t * 0x9E3779B9u);
-    const float inv_bc1 = (float)st.inv_bc1, inv_bc2 = (float)st.inv_bc2, eps = (float)a.eps, lr = (float)a.lr,
-                decay = c.decay ? (float)a.decay : 0.f;
-    const double b1 = a.b1, c1 = 1.0 - a.b1, b2 = a.b2, c2 = 1.0 - a.b2;
-    long long at;
-    const void* gp = grad_of(a, c, at);
-    float* __restrict__ p = c.param;
-    unsigned char* __restrict__ m8 = (unsigned char*)a.m + c.state_at;
-    unsigned char* __restrict__ v8 = (unsigned char*)a.v + c.state_at;
-    const int blocks = (c.count + ADAMW_BLOCK - 1) / ADAMW_BLOCK;
-    const long long block0 = c.state_at / ADAMW_BLOCK;
-    for (int i = threadIdx.x * 8; i < blocks * ADAMW_BLOCK; i += NT * 8) {
-        const long long block = block0 + i / ADAMW_BLOCK;
-        const u32x2 mc = *(const u32x2*)(m8 + i), vc = *(const u32x2*)(v8 + i);
-        const double ms = b1 * (double)a.m_scale[block], vs = b2 * (double)a.v_scale[block];
-        float g[8], pv[8];
-        const int n = min(8, c.count - i);              // may be below zero at a block's filled end
-        if (n == 8) {
+    const Scalars8 s{a.b1, (1.0 - a.b1) * st.coef, a.b2, (1.0 - a.b2) * st.coef * st.coef, st.inv_bc1, st.inv_bc2,
+                     (float)a.eps, (float)a.lr, c.decay ? (float)a.decay : 0.f, mix(a.seed + (unsigned)st.t * 0x9E3779B9u)};
 #pragma unroll
-            for (int k = 0; k < 8; k += 4) {
-                const f32x4 x = load_grad4(gp, at + i + k, a.grad_bf16), y = *(const f32x4_u*)(p + i + k);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    g[k + q] = x[q];
-                    pv[k + q] = y[q];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                g[k] = k < n ? load_grad(gp, at + i + k, a.grad_bf16) : 0.f;
-                pv[k] = k < n ? p[i + k] : 0.f;
-            }
-        }
-        float mf[8], vf[8];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            mf[4 * k] = __builtin_amdgcn_cvt_f32_fp8(mc[k], 0);
-            mf[4 * k + 1] = __builtin_amdgcn_cvt_f32_fp8(mc[k], 1);
-            mf[4 * k + 2] = __builtin_amdgcn_cvt_f32_fp8(mc[k], 2);
-            mf[4 * k + 3] = __builtin_amdgcn_cvt_f32_fp8(mc[k], 3);
-            vf[4 * k] = __builtin_amdgcn_cvt_f32_fp8(vc[k], 0);
-            vf[4 * k + 1] = __builtin_amdgcn_cvt_f32_fp8(vc[k], 1);
-            vf[4 * k + 2] = __builtin_amdgcn_cvt_f32_fp8(vc[k], 2);
-            vf[4 * k + 3] = __builtin_amdgcn_cvt_f32_fp8(vc[k], 3);
-        }
-        double m[8], v[8], mm = 0.0, vm = 0.0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const double gd = (double)g[k] * st.coef;
-            m[k] = fma(ms, (double)mf[k], c1 * gd);
-            v[k] = fma(vs, (double)vf[k], c2 * (gd * gd));
-            const double am = fabs(m[k]);
-            mm = (am > mm || am != am) ? am : mm;
-            vm = (v[k] > vm || v[k] != v[k]) ? v[k] : vm;
-            const float q = ((float)m[k] * inv_bc1) / (sqrtf((float)v[k] * inv_bc2) + eps);
-            pv[k] = fmaf(-lr, fmaf(decay, pv[k], q), pv[k]);
-        }
-        if (n == 8) {
-#pragma unroll
-            for (int k = 0; k < 8; k += 4) *(f32x4_u*)(p + i + k) = f32x4{pv[k], pv[k + 1], pv[k + 2], pv[k + 3]};
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (k < n) p[i + k] = pv[k];
-        }
-        const float new_ms = (float)(max16(mm) / 448.0), new_vs = (float)(max16(vm) / 448.0);
-        const double im = new_ms > 0.f || new_ms != new_ms ? 1.0 / (double)new_ms : 0.0,
-                     iv = new_vs > 0.f || new_vs != new_vs ? 1.0 / (double)new_vs : 0.0;
-        const unsigned pair = (unsigned)((unsigned long long)(c.state_at + i) >> 1);
-        u32x2 mo, vo;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            float y[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                y[q] = (float)(m[4 * k + q] * im);
-                y[q] = y[q] > 448.f ? 448.f : (y[q] < -448.f ? -448.f : y[q]);      // keeps a NaN
-            }
-            int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-            w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
-            mo[k] = (unsigned)w;
-            unsigned b = 0;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const unsigned h = mix((pair + 2 * k + q / 2) ^ key);
-                const double x = v[4 * k + q];
-                const float z = (float)(x * iv);
-                unsigned code = round_random(z, (q & 1) ? h >> 16 : h & 0xFFFFu);
-                code = code == 0 && x > 0.0 && new_vs > 0.f ? 1u : code;
-                if (z != z) code = 0x7Fu;
-                b |= code << (8 * q);
-            }
-            vo[k] = b;
-        }
-        *(u32x2*)(m8 + i) = mo;
-        *(u32x2*)(v8 + i) = vo;
-        if ((threadIdx.x & 15) == 0) {
-            a.m_scale[block] = new_ms;
-            a.v_scale[block] = new_vs;
-        }
+    for (int r = 0; r < R; ++r) {
+        const int i = i0 + r * 8 * NT;
+        if (c.count == ADAMW_CHUNK) step8<PAST, true>(e[r], a, c, i, 8, s);
+        else if (i < filled) step8<PAST, false>(e[r], a, c, i, c.count - i, s);
+        __builtin_amdgcn_sched_barrier(0);      // one after the other: together they take 154 registers
     }
-    step_done(a, st.t);
+    step_done(a, st);
 }
 
 }  // namespace
@@ -313,15 +427,26 @@ hipError_t adamw_set_pointers_launch(const AdamwPtrs& p, const void** dst, int n
 }
 
 hipError_t adamw_norm_launch(const AdamwArgs& a, double* partials, hipStream_t st) {
-    hipLaunchKernelGGL(norm_kernel, dim3((unsigned)a.num_partials), dim3(NT), 0, st, a, partials);
+    if (a.grad_bf16)
+        hipLaunchKernelGGL(norm_kernel<true>, dim3((unsigned)a.num_partials), dim3(NT), 0, st, a, partials);
+    else
+        hipLaunchKernelGGL(norm_kernel<false>, dim3((unsigned)a.num_partials), dim3(NT), 0, st, a, partials);
     return hipGetLastError();
 }
 
-hipError_t adamw_step_launch(const AdamwArgs& a, int state_bits, hipStream_t st) {
-    if (state_bits == 8)
-        hipLaunchKernelGGL(adamw8_kernel, dim3((unsigned)a.num_chunks), dim3(NT), 0, st, a);
-    else
-        hipLaunchKernelGGL(adamw32_kernel, dim3((unsigned)a.num_chunks), dim3(NT), 0, st, a);
+hipError_t adamw_step_launch(const AdamwArgs& a, int state_bits, bool past, hipStream_t st) {
+    const dim3 grid((unsigned)a.num_chunks), block(NT);
+#define ADAMW(K)                                                                                 \
+    if (a.grad_bf16 && past) hipLaunchKernelGGL((K<true, true>), grid, block, 0, st, a);         \
+    else if (a.grad_bf16) hipLaunchKernelGGL((K<true, false>), grid, block, 0, st, a);           \
+    else if (past) hipLaunchKernelGGL((K<false, true>), grid, block, 0, st, a);                  \
+    else hipLaunchKernelGGL((K<false, false>), grid, block, 0, st, a);
+    if (state_bits == 8) {
+        ADAMW(adamw8_kernel)
+    } else {
+        ADAMW(adamw32_kernel)
+    }
+#undef ADAMW
     return hipGetLastError();
 }
 

@@ -22,16 +22,18 @@ struct rst_adamw {
     AdamwChunk* d_chunks = nullptr;
     const void** d_ptrs = nullptr;
     double* d_partials = nullptr;
-    unsigned* d_ticket = nullptr;
+    unsigned* d_tickets = nullptr;
     ~rst_adamw() {
         (void)hipFree(d_chunks);
         (void)hipFree(d_ptrs);
         (void)hipFree(d_partials);
-        (void)hipFree(d_ticket);
+        (void)hipFree(d_tickets);
     }
 };
 
 namespace {
+
+constexpr size_t STREAMING_BYTES = 128u << 20;
 
 int step_args(rst_adamw* h, const char* who, int dtype, const rst_adamw_config* c, AdamwArgs& a) {
     const std::string name(who);
@@ -39,9 +41,9 @@ int step_args(rst_adamw* h, const char* who, int dtype, const rst_adamw_config* 
         return set_error(RST_ERR_UNSUPPORTED, name + ": gradients are float32 or bfloat16");
     if (!(c->beta_1 >= 0.0 && c->beta_1 < 1.0 && c->beta_2 >= 0.0 && c->beta_2 < 1.0))
         return set_error(RST_ERR_INVALID, name + ": beta_1 and beta_2 must lie in [0, 1)");
-    if (!std::isfinite(c->learning_rate) || !std::isfinite(c->weight_decay) || !(c->epsilon >= 0.0) ||
+    if (!std::isfinite(c->learning_rate) || !std::isfinite(c->weight_decay) || !(c->epsilon > 0.0) ||
         !std::isfinite(c->epsilon) || !(c->global_clipnorm >= 0.0))
-        return set_error(RST_ERR_INVALID, name + ": hyperparameters must be finite, epsilon and global_clipnorm not negative");
+        return set_error(RST_ERR_INVALID, name + ": hyperparameters must be finite, epsilon positive and global_clipnorm not negative");
     int dev = 0;
     RST_HIP_TRY(hipGetDevice(&dev));
     if (dev != h->device)
@@ -57,7 +59,7 @@ int step_args(rst_adamw* h, const char* who, int dtype, const rst_adamw_config* 
     a.v_scale = h->state.v_scale;
     a.iterations = h->state.iterations;
     a.global_norm = h->state.global_norm;
-    a.ticket = h->d_ticket;
+    a.tickets = h->d_tickets;
     a.partials = h->d_partials;
     a.num_partials = c->global_clipnorm > 0.0 ? std::min(h->num_chunks, ADAMW_MAX_PARTIALS) : 0;
     a.lr = c->learning_rate;
@@ -75,7 +77,8 @@ int step_args(rst_adamw* h, const char* who, int dtype, const rst_adamw_config* 
 int launch(rst_adamw* h, const AdamwArgs& a, hipStream_t st) {
     if (h->num_chunks == 0) return RST_OK;
     if (a.num_partials > 0) RST_HIP_TRY(adamw_norm_launch(a, h->d_partials, st));
-    RST_HIP_TRY(adamw_step_launch(a, h->bits, st));
+    const bool past = h->num_elements * (h->bits == 8 ? 14 : 26) > STREAMING_BYTES;
+    RST_HIP_TRY(adamw_step_launch(a, h->bits, past, st));
     return RST_OK;
 }
 
@@ -114,14 +117,14 @@ int create(const rst_adamw_tensor* tensors, int n, int bits, const rst_adamw_sta
     h->num_elements = elements;
     h->state = *state;
     if (chunks.empty()) return RST_OK;
-    const unsigned zero = 0;
+    const std::vector<unsigned> zeros((1 + (chunks.size() + ADAMW_TICKETS - 1) / ADAMW_TICKETS) * ADAMW_TICKET_STRIDE, 0u);
     if (hipMalloc(&h->d_chunks, chunks.size() * sizeof(AdamwChunk)) != hipSuccess ||
         hipMalloc(&h->d_ptrs, n * sizeof(void*)) != hipSuccess ||
         hipMalloc(&h->d_partials, ADAMW_MAX_PARTIALS * sizeof(double)) != hipSuccess ||
-        hipMalloc(&h->d_ticket, sizeof(unsigned)) != hipSuccess)
+        hipMalloc(&h->d_tickets, zeros.size() * sizeof(unsigned)) != hipSuccess)
         return set_error(RST_ERR_ALLOC, "rst_adamw_create: device allocation failed");
     RST_HIP_TRY(hipMemcpy(h->d_chunks, chunks.data(), chunks.size() * sizeof(AdamwChunk), hipMemcpyHostToDevice));
-    RST_HIP_TRY(hipMemcpy(h->d_ticket, &zero, sizeof(zero), hipMemcpyHostToDevice));
+    RST_HIP_TRY(hipMemcpy(h->d_tickets, zeros.data(), zeros.size() * sizeof(unsigned), hipMemcpyHostToDevice));
     return RST_OK;
 }
 

@@ -26,6 +26,7 @@ struct GroupNormArgs {
 
 size_t group_norm_workspace_bytes(int batch, long hw, int C, int G);
 bool group_norm_supported(int batch, long hw, int C, int G);
+size_t group_norm_bwd_workspace_bytes(int batch, long hw, int C, int G);
 hipError_t group_norm_launch(const GroupNormArgs& a, hipStream_t st);
 hipError_t group_norm_bwd_launch(const GroupNormArgs& a, hipStream_t st);
 

@@ -1117,6 +1117,10 @@ size_t rst_group_norm_workspace_size(int batch, int hw, int channels, int groups
     return group_norm_workspace_bytes(batch, hw, channels, groups);
 }
 
+size_t rst_group_norm_backward_workspace_size(int batch, int hw, int channels, int groups) {
+    return group_norm_bwd_workspace_bytes(batch, hw, channels, groups);
+}
+
 static int group_norm_check(const char* who, int dtype, int batch, int hw, int channels, int groups, int activation) {
     const std::string name(who);
     if (batch < 0 || hw < 0 || channels <= 0 || groups <= 0 || channels % groups != 0)
@@ -1136,8 +1140,9 @@ int rst_group_norm(const void* x, int dtype, int batch, int hw, int channels, in
     const int rc = group_norm_check("rst_group_norm", dtype, batch, hw, channels, groups, activation);
     if (rc != RST_OK) return rc;
     if (batch == 0 || hw == 0) return RST_OK;
-    if (x == nullptr || scale == nullptr || bias == nullptr || y == nullptr || workspace == nullptr ||
-        ((size_t)workspace & 15) != 0 || !(eps >= 0.f))
+    if (x == nullptr || scale == nullptr || bias == nullptr || y == nullptr || !(eps >= 0.f) ||
+        ((size_t)workspace & 15) != 0 ||
+        (workspace == nullptr && group_norm_workspace_bytes(batch, hw, channels, groups) != 0))
         return fail(RST_ERR_INVALID, "rst_group_norm: null pointer, workspace not aligned to 16 bytes or negative eps");
     GroupNormArgs a{};
     a.x = x;
@@ -1168,7 +1173,8 @@ int rst_group_norm_backward(const void* x, const void* dy, int dtype, int batch,
     if (dscale == nullptr || dbias == nullptr)
         return fail(RST_ERR_INVALID, "rst_group_norm_backward: null pointer");
     if (!empty && (x == nullptr || dy == nullptr || scale == nullptr || bias == nullptr || mean == nullptr ||
-                   rstd == nullptr || dx == nullptr || workspace == nullptr || ((size_t)workspace & 15) != 0))
+                   rstd == nullptr || dx == nullptr || ((size_t)workspace & 15) != 0 ||
+                   (workspace == nullptr && group_norm_bwd_workspace_bytes(batch, hw, channels, groups) != 0)))
         return fail(RST_ERR_INVALID, "rst_group_norm_backward: null pointer or workspace not aligned to 16 bytes");
     GroupNormArgs a{};
     a.x = x;

@@ -43,13 +43,13 @@ class AdamW:
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits!r}")
         if global_clipnorm is not None and not global_clipnorm > 0.0:
-            raise ValueError(f"global_clipnorm must be positive or None, got {global_clipnorm!r}")
+            raise ValueError(f"global_clipnorm must be positive and finite, or None, got {global_clipnorm!r}")
         self.learning_rate, self.weight_decay = float(learning_rate), float(weight_decay)
         self.beta_1, self.beta_2, self.epsilon = float(beta_1), float(beta_2), float(epsilon)
         self.global_clipnorm = None if global_clipnorm is None else float(global_clipnorm)
         self.state_bits, self.seed = int(state_bits), int(seed)
-        self._handle = None
-        self._config = _lib.RstAdamwConfig()
+        self._handle = self._owner = None
+        self._config, self._config_of = _lib.RstAdamwConfig(), None
         self._check_config()
 
     def __del__(self):
@@ -61,14 +61,21 @@ class AdamW:
             pass
 
     def _check_config(self):
-        c, clip = self._config, self.global_clipnorm
+        clip = self.global_clipnorm
+        of = (self.learning_rate, self.weight_decay, self.beta_1, self.beta_2, self.epsilon, clip, self.seed)
+        if of == self._config_of:
+            return self._config
+        c = _lib.RstAdamwConfig()
         c.learning_rate, c.weight_decay, c.epsilon = self.learning_rate, self.weight_decay, self.epsilon
         c.beta_1, c.beta_2, c.seed = self.beta_1, self.beta_2, self.seed & 0xFFFFFFFF
         c.global_clipnorm = 0.0 if clip is None else clip
         if not (0.0 <= c.beta_1 < 1.0 and 0.0 <= c.beta_2 < 1.0):
             raise ValueError(f"beta_1 and beta_2 must lie in [0, 1), got {c.beta_1} and {c.beta_2}")
-        if not (math.isfinite(c.learning_rate) and math.isfinite(c.weight_decay) and 0.0 <= c.epsilon < math.inf):
-            raise ValueError("learning_rate, weight_decay and epsilon must be finite, epsilon not negative")
+        if not (math.isfinite(c.learning_rate) and math.isfinite(c.weight_decay) and 0.0 < c.epsilon < math.inf):
+            raise ValueError("learning_rate, weight_decay and epsilon must be finite, epsilon positive")
+        if not 0.0 <= c.global_clipnorm < math.inf:
+            raise ValueError(f"global_clipnorm must be positive and finite, or None, got {clip!r}")
+        self._config, self._config_of = c, of
         return c
 
     # ------------------------------------------------------------------ state
@@ -109,6 +116,7 @@ class AdamW:
         self._bucket_size = max((o + n for o, n in zip(offsets, counts)), default=0)
         n, blocks = sum(counts), sum((c + BLOCK - 1) // BLOCK for c in counts)
         self.device = torch.device(device)
+        self._index = self.device.index if self.device.index is not None else torch.cuda.current_device()
         with torch.cuda.device(self.device):
             if self.state_bits == 32:
                 self.m, self.v = torch.zeros(n, device=device), torch.zeros(n, device=device)
@@ -187,12 +195,15 @@ class AdamW:
         """One step on the current stream. ``gradients``: the bucket (one contiguous tensor, float32 or bfloat16), or a
         list of one contiguous tensor per variable, all of one dtype."""
         self._require_built()
-        lib, config = _lib.load(), self._check_config()
+        if torch.cuda.current_device() != self._index:
+            with torch.cuda.device(self.device):
+                return self.apply_gradients(gradients)
+        lib, config, stream = _lib.load(), self._check_config(), _lib.device_stream(self._index)
         if isinstance(gradients, torch.Tensor):
             if gradients.numel() != self._bucket_size:
                 raise ValueError(f"the gradient bucket must have {self._bucket_size} elements, got {gradients.numel()}")
             pointer, dtype = self._gradient(gradients)
-            step = lambda st: lib.rst_adamw_step(self._handle, pointer, dtype, ctypes.byref(config), st)  # noqa: E731
+            _lib.check(lib.rst_adamw_step(self._handle, pointer, dtype, ctypes.byref(config), stream))
         else:
             gradients = list(gradients)
             if [-1 if g is None else g.numel() for g in gradients] != self._counts:
@@ -202,13 +213,7 @@ class AdamW:
             if any(d != dtype for _, d in rows):
                 raise ValueError("gradients must all be float32 or all bfloat16")
             pointers = (ctypes.c_void_p * len(rows))(*[p for p, _ in rows])
-            step = lambda st: lib.rst_adamw_step_tensors(self._handle, pointers, len(rows), dtype,  # noqa: E731
-                                                         ctypes.byref(config), st)
-        if torch.cuda.current_device() == self.device.index:
-            _lib.check(step(_lib.stream_ptr()))
-        else:
-            with torch.cuda.device(self.device):
-                _lib.check(step(_lib.stream_ptr()))
+            _lib.check(lib.rst_adamw_step_tensors(self._handle, pointers, len(rows), dtype, ctypes.byref(config), stream))
 
     def _gradient(self, g: torch.Tensor) -> Tuple[int, int]:
         if g.device != self.device:

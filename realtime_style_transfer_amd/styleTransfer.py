@@ -299,33 +299,38 @@ def instance_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, eps:
     return y
 
 
-def _group_norm_check(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, groups: int, activation: str, *more):
+_GN_DTYPES = {torch.float32: _lib.DTYPES["float32"], torch.bfloat16: _lib.DTYPES["bfloat16"]}
+
+
+def _group_norm_check(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, groups: int, activation: str, more):
     """The shared argument checks of group_norm and group_norm_gradients -> (dtype, activation, per_image)."""
     if x.dim() != 4:
         raise ValueError(f"x must be (B,H,W,C), got {tuple(x.shape)}")
-    B, C = x.shape[0], x.shape[3]
-    if x.dtype is not torch.float32 and x.dtype is not torch.bfloat16:
+    B, _, _, C = x.shape
+    dtype, act = _GN_DTYPES.get(x.dtype), _lib.ACTIVATIONS.get(activation)
+    if dtype is None:
         raise ValueError(f"x must be float32 or bfloat16, got {x.dtype}")
     if groups < 1 or C < 1 or C % groups != 0:
         raise ValueError(f"{groups} groups do not divide {C} channels")
-    if activation not in _lib.ACTIVATIONS:
+    if act is None:
         raise ValueError(f"unknown activation {activation!r}; supported: {sorted(_lib.ACTIVATIONS)}")
     per_image = scale.dim() == 2
     shape = (B, C) if per_image else (C,)
     if scale.shape != shape or bias.shape != shape:
         raise ValueError(f"scale and bias must both be (C,) = ({C},) or (B,C) = ({B},{C}), got {tuple(scale.shape)} and "
                          f"{tuple(bias.shape)}")
-    if not x.is_cuda:
+    if scale.dtype is not torch.float32 or bias.dtype is not torch.float32:
+        raise ValueError(f"scale and bias must be float32, got {scale.dtype} and {bias.dtype}")
+    device = x.device
+    if device.type != 'cuda':
         raise ValueError("librst operates on device tensors; got a CPU tensor")
-    for t in (scale, bias) + more:
-        if t.device != x.device:
-            raise ValueError(f"x is on {x.device}, another tensor on {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
+    grad = torch.is_grad_enabled()
+    for t in (x, scale, bias, *more):
+        if t.device != device:
+            raise ValueError(f"x is on {device}, another tensor on {t.device}")
+        if grad and t.requires_grad:
             raise ValueError("group_norm is not recorded by autograd: detach its inputs and use group_norm_gradients")
-    for t in (scale, bias):
-        if t.dtype is not torch.float32:
-            raise ValueError(f"scale and bias must be float32, got {t.dtype}")
-    return _lib.DTYPES["float32" if x.dtype is torch.float32 else "bfloat16"], _lib.ACTIVATIONS[activation], per_image
+    return dtype, act, per_image
 
 
 def group_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, groups: int, eps: float = CIN_EPS,
@@ -336,20 +341,24 @@ def group_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, groups:
     x (B,H,W,C) float32 or bfloat16; scale and bias (C,), or (B,C) per image (style parameters), float32; activation
     "linear", "relu", "swish" or "hard_swish". groups == C is ``instance_norm``. Returns y like x; with
     ``return_statistics`` (y, mean, rstd), the statistics (B, groups) float32 that ``group_norm_gradients`` takes."""
-    dtype, act, per_image = _group_norm_check(x, scale, bias, groups, activation, x)
+    dtype, act, per_image = _group_norm_check(x, scale, bias, groups, activation, ())
     B, H, W, C = x.shape
-    x, scale, bias = x.contiguous(), scale.contiguous(), bias.contiguous()
-    if torch.cuda.current_device() != x.device.index:
-        with torch.cuda.device(x.device):
+    index = x.device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
             return group_norm(x, scale, bias, groups, eps, activation, return_statistics)
+    x, scale, bias = x.contiguous(), scale.contiguous(), bias.contiguous()
     lib = _lib.load()
     y = torch.empty_like(x)
-    stats = torch.empty((2, B, groups), dtype=torch.float32, device=x.device)
-    ws = torch.empty(lib.rst_group_norm_workspace_size(B, H * W, C, groups), dtype=torch.uint8, device=x.device)
-    mean, rstd = stats.unbind(0)
+    need = lib.rst_group_norm_workspace_size(B, H * W, C, groups)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    mean = rstd = None
+    if return_statistics:
+        mean, rstd = scale.new_empty((2, B, groups)).unbind()
     _lib.check(lib.rst_group_norm(x.data_ptr(), dtype, B, H * W, C, groups, scale.data_ptr(), bias.data_ptr(),
-                                  per_image, eps, act, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(),
-                                  _lib.stream_ptr()))
+                                  per_image, eps, act, y.data_ptr(), None if mean is None else mean.data_ptr(),
+                                  None if rstd is None else rstd.data_ptr(), None if ws is None else ws.data_ptr(),
+                                  _lib.device_stream(index)))
     return (y, mean, rstd) if return_statistics else y
 
 
@@ -357,24 +366,26 @@ def group_norm_gradients(x: torch.Tensor, dy: torch.Tensor, scale: torch.Tensor,
                          rstd: torch.Tensor, groups: int, activation: str = "linear"):
     """The gradients of ``group_norm``: from dy = d loss / d y (like x) and the forward's statistics -> (dx like x, dscale,
     dbias shaped as scale; sums over the batch where the affine is shared)."""
-    dtype, act, per_image = _group_norm_check(x, scale, bias, groups, activation, x, dy, mean, rstd)
+    dtype, act, per_image = _group_norm_check(x, scale, bias, groups, activation, (dy, mean, rstd))
     B, H, W, C = x.shape
     if dy.shape != x.shape or dy.dtype is not x.dtype:
         raise ValueError(f"dy must be like x, {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
     for t in (mean, rstd):
         if t.shape != (B, groups) or t.dtype is not torch.float32:
             raise ValueError(f"mean and rstd must be ({B},{groups}) float32, got {tuple(t.shape)} {t.dtype}")
+    index = x.device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return group_norm_gradients(x, dy, scale, bias, mean, rstd, groups, activation)
     x, dy, scale, bias = x.contiguous(), dy.contiguous(), scale.contiguous(), bias.contiguous()
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    if torch.cuda.current_device() != x.device.index:
-        with torch.cuda.device(x.device):
-            return group_norm_gradients(x, dy, scale, bias, mean, rstd, groups, activation)
     lib = _lib.load()
     dx = torch.empty_like(x)
-    dscale, dbias = torch.empty((2,) + tuple(scale.shape), dtype=torch.float32, device=x.device).unbind(0)
-    ws = torch.empty(lib.rst_group_norm_workspace_size(B, H * W, C, groups), dtype=torch.uint8, device=x.device)
+    dscale, dbias = scale.new_empty((2,) + scale.shape).unbind()
+    need = lib.rst_group_norm_backward_workspace_size(B, H * W, C, groups)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _lib.check(lib.rst_group_norm_backward(x.data_ptr(), dy.data_ptr(), dtype, B, H * W, C, groups, scale.data_ptr(),
                                            bias.data_ptr(), per_image, mean.data_ptr(), rstd.data_ptr(), act,
-                                           dx.data_ptr(), dscale.data_ptr(), dbias.data_ptr(), ws.data_ptr(),
-                                           _lib.stream_ptr()))
+                                           dx.data_ptr(), dscale.data_ptr(), dbias.data_ptr(),
+                                           None if ws is None else ws.data_ptr(), _lib.device_stream(index)))
     return dx, dscale, dbias

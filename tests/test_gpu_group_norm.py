@@ -257,7 +257,8 @@ def test_in_place_through_the_c_interface():
     x, scale, bias, dy = _inputs((2, 40, 50, 24, 3), torch.float32, False)
     y, mean, rstd = gn(x, scale, bias, 3, activation="relu", return_statistics=True)
     dx, ds, db = grad(x, dy, scale, bias, mean, rstd, 3, "relu")
-    ws = torch.empty(lib.rst_group_norm_workspace_size(2, 2000, 24, 3), dtype=torch.uint8, device='cuda')
+    need = max(lib.rst_group_norm_workspace_size(2, 2000, 24, 3), lib.rst_group_norm_backward_workspace_size(2, 2000, 24, 3))
+    ws = torch.empty(need, dtype=torch.uint8, device='cuda')
     d2, s2, b2 = dy.clone(), torch.empty_like(ds), torch.empty_like(db)
     L.check(lib.rst_group_norm_backward(x.data_ptr(), d2.data_ptr(), 0, 2, 2000, 24, 3, scale.data_ptr(),
                                         bias.data_ptr(), 0, mean.data_ptr(), rstd.data_ptr(), 1, d2.data_ptr(),

@@ -60,7 +60,7 @@ def test_backward_refusals():
     keep, x = _buffer()
     ok = [x, x, F32, 1, 4, 4, 2, x, x, 0, x, x, 0, x, x, x, x, None]
     for at, bad, code in [(0, None, 1), (1, None, 1), (7, None, 1), (8, None, 1), (10, None, 1), (11, None, 1),
-                          (13, None, 1), (14, None, 1), (15, None, 1), (16, None, 1), (16, x + 8, 1), (6, 3, 1),
+                          (13, None, 1), (14, None, 1), (15, None, 1), (16, x + 8, 1), (6, 3, 1),
                           (2, 7, 2), (12, 9, 2), (3, -1, 1)]:
         args = list(ok)
         args[at] = bad
@@ -70,10 +70,20 @@ def test_backward_refusals():
 
 def test_workspace_size():
     lib = _lib()
-    size = lib.rst_group_norm_workspace_size
-    assert size(0, 4, 4, 2) > 0 and size(1, 4, 4, 3) > 0            # refused shapes still get a size
-    assert size(1, 28800, 128, 32) > 0
-    assert size(4, 480 * 960, 32, 8) < 64 << 20                      # partial sums, not another tensor
+    for size in (lib.rst_group_norm_workspace_size, lib.rst_group_norm_backward_workspace_size):
+        assert size(0, 4, 4, 2) == 0 and size(1, 4, 4, 3) == 0 and size(1, 4, 0, 1) == 0
+        assert size(1, 450, 96, 8) == 0                              # one launch holds it in registers
+        assert 0 < size(1, 28800, 128, 32) < 64 << 20
+        assert 0 < size(4, 480 * 960, 32, 8) < 64 << 20              # partial sums, not another tensor
+    assert lib.rst_group_norm_backward_workspace_size(3, 450, 96, 8) == 3 * 96 * 16     # a shared affine's sums
+
+
+def test_a_workspace_that_is_needed_has_to_be_there():
+    lib = _lib()
+    keep, x = _buffer()
+    assert lib.rst_group_norm(x, F32, 1, 28800, 128, 32, x, x, 0, 1e-5, 0, x, None, None, None, None) == L.RST_ERR_INVALID
+    assert lib.rst_group_norm_backward(x, x, F32, 1, 28800, 128, 32, x, x, 0, x, x, 0, x, x, x, None, None) == \
+        L.RST_ERR_INVALID
 
 
 def test_python_refusals_without_a_device():
