@@ -194,6 +194,7 @@ __global__ __launch_bounds__(NT) void adamw32_kernel(AdamwArgs a) {
     if (vectors > 0) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
+            if (r * NT >= vectors) break;
             const int i = full || i0 / 4 + r * NT < vectors ? i0 + r * 4 * NT : 0;
             gv[r] = load_grad4<BF16, PAST>(g, at + i);
             pv[r] = load<PAST, f32x4_u>(p, 4ll * i);
@@ -323,7 +324,7 @@ struct Scalars8 {
 };
 
 // Their step: 16 lanes are a block
-template <bool PAST, bool FULL>
+template <bool PAST>
 __device__ __forceinline__ void step8(Eight& e, const AdamwArgs& a, const AdamwChunk& c, int i, int n, const Scalars8& s) {
     float mf[8], vf[8];
 #pragma unroll
@@ -349,14 +350,14 @@ __device__ __forceinline__ void step8(Eight& e, const AdamwArgs& a, const AdamwC
         const float q = quotient((float)m[k], (float)v[k], s.inv_bc1, s.inv_bc2, s.eps);
         e.p[k] = fmaf(-s.lr, fmaf(s.decay, e.p[k], q), e.p[k]);
     }
-    if constexpr (FULL) {
+    if (n >= 8) {
 #pragma unroll
         for (int k = 0; k < 8; k += 4)
             store<PAST, f32x4_u>(c.param, 4ll * (i + k), f32x4{e.p[k], e.p[k + 1], e.p[k + 2], e.p[k + 3]});
     } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-            if (k < n) c.param[i + k] = e.p[k];
+            if (k < n) store<false, float>(c.param, 4ll * (i + k), e.p[k]);
     }
     const float new_ms = scale_of(max16(mm)), new_vs = scale_of(max16(vm));
     const double im = inverse(new_ms), iv = inverse(new_vs);
@@ -400,7 +401,7 @@ __global__ __launch_bounds__(NT, 3) void adamw8_kernel(AdamwArgs a) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int i = i0 + r * 8 * NT;
-        if (c.count == ADAMW_CHUNK) load8<BF16, PAST, true>(e[r], a, c, g, at, i, 8);
+        if (i + 8 <= c.count) load8<BF16, PAST, true>(e[r], a, c, g, at, i, 8);
         else if (i < filled) load8<BF16, PAST, false>(e[r], a, c, g, at, i, c.count - i);
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -412,8 +413,7 @@ __global__ __launch_bounds__(NT, 3) void adamw8_kernel(AdamwArgs a) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int i = i0 + r * 8 * NT;
-        if (c.count == ADAMW_CHUNK) step8<PAST, true>(e[r], a, c, i, 8, s);
-        else if (i < filled) step8<PAST, false>(e[r], a, c, i, c.count - i, s);
+        if (i < filled) step8<PAST>(e[r], a, c, i, c.count - i, s);
         __builtin_amdgcn_sched_barrier(0);      // one after the other: together they take 154 registers
     }
     step_done(a, st);

@@ -17,7 +17,8 @@ using namespace rst;
 
 struct rst_adamw {
     int device = 0, bits = 32, num_tensors = 0, num_chunks = 0;
-    size_t num_blocks = 0, num_elements = 0;
+    size_t num_blocks = 0;
+    bool past = false;                 // the step's data does not stay in the caches
     rst_adamw_state state{};
     AdamwChunk* d_chunks = nullptr;
     const void** d_ptrs = nullptr;
@@ -33,22 +34,27 @@ struct rst_adamw {
 
 namespace {
 
+// A step that touches more than half of the 256 MB Infinity Cache loads and stores past it (12 M elements, 32-bit states
+// 70 us, through it 80; 6 M 38.9 and 44.4)
 constexpr size_t STREAMING_BYTES = 128u << 20;
+constexpr size_t MAX_ELEMENTS = (size_t)1 << 36;     // 256 GB of variables
 
 int step_args(rst_adamw* h, const char* who, int dtype, const rst_adamw_config* c, AdamwArgs& a) {
-    const std::string name(who);
-    if (dtype != RST_DTYPE_FLOAT32 && dtype != RST_DTYPE_BFLOAT16)
-        return set_error(RST_ERR_UNSUPPORTED, name + ": gradients are float32 or bfloat16");
-    if (!(c->beta_1 >= 0.0 && c->beta_1 < 1.0 && c->beta_2 >= 0.0 && c->beta_2 < 1.0))
-        return set_error(RST_ERR_INVALID, name + ": beta_1 and beta_2 must lie in [0, 1)");
-    if (!std::isfinite(c->learning_rate) || !std::isfinite(c->weight_decay) || !(c->epsilon > 0.0) ||
-        !std::isfinite(c->epsilon) || !(c->global_clipnorm >= 0.0))
-        return set_error(RST_ERR_INVALID, name + ": hyperparameters must be finite, epsilon positive and global_clipnorm not negative");
-    int dev = 0;
+    const char* what = nullptr;      // (no string is made where nothing is wrong)
+    int dev = 0, code = RST_ERR_INVALID;
     RST_HIP_TRY(hipGetDevice(&dev));
-    if (dev != h->device)
-        return set_error(RST_ERR_INVALID, name + ": made on device " + std::to_string(h->device) +
-                                              ", called on device " + std::to_string(dev));
+    if (dtype != RST_DTYPE_FLOAT32 && dtype != RST_DTYPE_BFLOAT16) {
+        what = "gradients are float32 or bfloat16";
+        code = RST_ERR_UNSUPPORTED;
+    } else if (!(c->beta_1 >= 0.0 && c->beta_1 < 1.0 && c->beta_2 >= 0.0 && c->beta_2 < 1.0)) {
+        what = "beta_1 and beta_2 must lie in [0, 1)";
+    } else if (!std::isfinite(c->learning_rate) || !std::isfinite(c->weight_decay) || !(c->epsilon > 0.0) ||
+               !std::isfinite(c->epsilon) || !(c->global_clipnorm >= 0.0) || !std::isfinite(c->global_clipnorm)) {
+        what = "hyperparameters must be finite, epsilon positive and global_clipnorm not negative";
+    } else if (dev != h->device) {
+        what = "called on another device than the handle was made on";
+    }
+    if (what != nullptr) return set_error(code, std::string(who) + ": " + what);
     a.chunks = h->d_chunks;
     a.grad_ptrs = h->d_ptrs;
     a.grad_bf16 = dtype == RST_DTYPE_BFLOAT16;
@@ -77,25 +83,39 @@ int step_args(rst_adamw* h, const char* who, int dtype, const rst_adamw_config* 
 int launch(rst_adamw* h, const AdamwArgs& a, hipStream_t st) {
     if (h->num_chunks == 0) return RST_OK;
     if (a.num_partials > 0) RST_HIP_TRY(adamw_norm_launch(a, h->d_partials, st));
-    const bool past = h->num_elements * (h->bits == 8 ? 14 : 26) > STREAMING_BYTES;
-    RST_HIP_TRY(adamw_step_launch(a, h->bits, past, st));
+    RST_HIP_TRY(adamw_step_launch(a, h->bits, h->past, st));
     return RST_OK;
+}
+
+// Elements per workgroup. 32-bit states: one vector per thread where the step streams through HBM (the workgroups' reads
+// then sweep closely: 48 M elements 217 us, with 4096 252; 12 M 60 and 68), four where latency counts (2.7 M with
+// clipping 17.6 us, with 1024 20.7). 8-bit states: two rounds of eight per thread pay for large steps (48 M 181 us, with
+// one 193), one for small (12 M 39.5 us, with two 43.4; 2.7 M 18.7 and 19.0).
+size_t chunk_size(size_t elements, int bits, bool past) {
+    if (bits == 32) return past ? ADAMW_CHUNK / 4 : ADAMW_CHUNK;
+    return elements < ((size_t)16 << 20) ? ADAMW_CHUNK / 2 : ADAMW_CHUNK;
 }
 
 int create(const rst_adamw_tensor* tensors, int n, int bits, const rst_adamw_state* state, rst_adamw* h) {
     std::vector<AdamwChunk> chunks;
-    size_t blocks = 0, elements = 0;
+    size_t blocks = 0, elements = 0, total = 0;
+    for (int k = 0; k < n; ++k) {
+        if (tensors[k].count > MAX_ELEMENTS || (total += tensors[k].count) > MAX_ELEMENTS)
+            return set_error(RST_ERR_INVALID, "rst_adamw_create: more elements than a device holds");
+    }
+    h->past = total * (bits == 8 ? 14 : 26) > STREAMING_BYTES;
+    const size_t chunk = chunk_size(total, bits, h->past);
+    chunks.reserve(total / chunk + n);
     for (int k = 0; k < n; ++k) {
         const rst_adamw_tensor& t = tensors[k];
         if (t.count != 0 && t.param == nullptr) return set_error(RST_ERR_INVALID, "rst_adamw_create: null variable");
-        if (t.count > ((size_t)1 << 40)) return set_error(RST_ERR_INVALID, "rst_adamw_create: variable too large");
-        for (size_t i = 0; i < t.count; i += ADAMW_CHUNK) {
+        for (size_t i = 0; i < t.count; i += chunk) {
             AdamwChunk c{};
             c.param = t.param + i;
             c.grad_at = (long long)(t.grad_offset + i);
             c.tensor_at = (long long)i;
             c.state_at = (long long)(bits == 8 ? blocks * ADAMW_BLOCK + i : elements + i);
-            c.count = (int)std::min((size_t)ADAMW_CHUNK, t.count - i);
+            c.count = (int)std::min(chunk, t.count - i);
             c.tensor = k;
             c.decay = t.decay != 0;
             chunks.push_back(c);
@@ -103,7 +123,6 @@ int create(const rst_adamw_tensor* tensors, int n, int bits, const rst_adamw_sta
         blocks += (t.count + ADAMW_BLOCK - 1) / ADAMW_BLOCK;
         elements += t.count;
     }
-    if (chunks.size() >= (size_t)1 << 31) return set_error(RST_ERR_UNSUPPORTED, "rst_adamw_create: too many elements");
     if (elements != 0 && (state->m == nullptr || state->v == nullptr ||
                           (bits == 8 && (state->m_scale == nullptr || state->v_scale == nullptr))))
         return set_error(RST_ERR_INVALID, "rst_adamw_create: null state");
@@ -114,7 +133,6 @@ int create(const rst_adamw_tensor* tensors, int n, int bits, const rst_adamw_sta
     h->num_tensors = n;
     h->num_chunks = (int)chunks.size();
     h->num_blocks = blocks;
-    h->num_elements = elements;
     h->state = *state;
     if (chunks.empty()) return RST_OK;
     const std::vector<unsigned> zeros((1 + (chunks.size() + ADAMW_TICKETS - 1) / ADAMW_TICKETS) * ADAMW_TICKET_STRIDE, 0u);

@@ -53,7 +53,9 @@ __device__ __forceinline__ double2 moments(double2 s, double inv_n, float eps) {
     const double mean = s.x * inv_n;
     double var = s.y * inv_n - mean * mean;
     var = var < 0.0 ? 0.0 : var;          // keeps a NaN
-    return make_double2(mean, 1.0 / sqrt(var + (double)eps));
+    // one Newton step on the hardware's 1 / sqrt: about one unit in the last place, where 0 and infinity keep theirs
+    const double d = var + (double)eps, r = __builtin_amdgcn_rsq(d), s1 = fma(0.5 * r, fma(-d * r, r, 1.0), r);
+    return make_double2(mean, s1 == s1 ? s1 : r);
 }
 
 template <int ACT>

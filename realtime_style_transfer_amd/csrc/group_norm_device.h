@@ -180,13 +180,26 @@ __device__ __forceinline__ int team(int threads, int n) {
     return n >= threads ? 1 : min(64, 1 << (31 - __clz(threads / n)));
 }
 
-__device__ __forceinline__ double2 team_sum(double2 v, int t) {
-    for (int o = t / 2; o > 0; o >>= 1) {
-        v.x += __shfl_xor(v.x, o);
-        v.y += __shfl_xor(v.y, o);
-    }
+// Lane permutations within a row on the halves of a double: the chain of cross-lane reads through LDS that __shfl_xor is
+// would take most of a small sum's time
+template <int CTRL>
+__device__ __forceinline__ double row_permuted(double v) {
+    const long long b = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)(b & 0xFFFFFFFFll), CTRL, 0xF, 0xF, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xF, 0xF, true);
+    return __longlong_as_double(((long long)hi << 32) | (unsigned)lo);
+}
+// Every member of a team gets its sum
+__device__ __forceinline__ double team_sum(double v, int t) {
+    if (t >= 2) v += row_permuted<0xB1>(v);      // lanes xor 1
+    if (t >= 4) v += row_permuted<0x4E>(v);      // lanes xor 2
+    if (t >= 8) v += row_permuted<0x141>(v);     // the half row mirrored
+    if (t >= 16) v += row_permuted<0x140>(v);    // the row mirrored
+    if (t >= 32) v += __shfl_xor(v, 16);
+    if (t >= 64) v += __shfl_xor(v, 32);
     return v;
 }
+__device__ __forceinline__ double2 team_sum(double2 v, int t) { return make_double2(team_sum(v.x, t), team_sum(v.y, t)); }
 
 // Sums by a team (member j of t) over the rows of red [rows][stride], columns lo .. lo + width
 __device__ __forceinline__ double2 team_block_sum(const double2* red, int rows, int stride, int lo, int width, int j, int t) {

@@ -1122,16 +1122,19 @@ size_t rst_group_norm_backward_workspace_size(int batch, int hw, int channels, i
 }
 
 static int group_norm_check(const char* who, int dtype, int batch, int hw, int channels, int groups, int activation) {
-    const std::string name(who);
-    if (batch < 0 || hw < 0 || channels <= 0 || groups <= 0 || channels % groups != 0)
-        return fail(RST_ERR_INVALID, name + ": batch and hw must not be negative, groups must divide the channels");
-    if (dtype != RST_DTYPE_FLOAT32 && dtype != RST_DTYPE_BFLOAT16)
-        return fail(RST_ERR_UNSUPPORTED, name + ": tensors are float32 or bfloat16");
-    if (activation < RST_ACT_LINEAR || activation > RST_ACT_HARD_SWISH)
-        return fail(RST_ERR_UNSUPPORTED, name + ": unknown activation");
-    if (!group_norm_supported(batch, hw, channels, groups))
-        return fail(RST_ERR_UNSUPPORTED, name + ": too many workgroups for one launch");
-    return RST_OK;
+    const char* what = nullptr;      // (no string is made where nothing is wrong)
+    int code = RST_ERR_UNSUPPORTED;
+    if (batch < 0 || hw < 0 || channels <= 0 || groups <= 0 || channels % groups != 0) {
+        what = "batch and hw must not be negative, groups must divide the channels";
+        code = RST_ERR_INVALID;
+    } else if (dtype != RST_DTYPE_FLOAT32 && dtype != RST_DTYPE_BFLOAT16) {
+        what = "tensors are float32 or bfloat16";
+    } else if (activation < RST_ACT_LINEAR || activation > RST_ACT_HARD_SWISH) {
+        what = "unknown activation";
+    } else if (!group_norm_supported(batch, hw, channels, groups)) {
+        what = "too many workgroups for one launch";
+    }
+    return what == nullptr ? RST_OK : fail(code, std::string(who) + ": " + what);
 }
 
 int rst_group_norm(const void* x, int dtype, int batch, int hw, int channels, int groups, const float* scale,

@@ -17,7 +17,7 @@ def _lib():
 
 def test_hyperparameters():
     for bad in (dict(state_bits=16), dict(global_clipnorm=0.0), dict(global_clipnorm=-1.0), dict(beta_1=1.0),
-                dict(beta_2=-0.1), dict(epsilon=-1e-8), dict(learning_rate=float('nan')),
+                dict(beta_2=-0.1), dict(epsilon=0.0), dict(epsilon=-1e-8), dict(global_clipnorm=float('inf')), dict(learning_rate=float('nan')),
                 dict(weight_decay=float('inf'))):
         with pytest.raises(ValueError):
             AdamW(**bad)
@@ -58,7 +58,8 @@ def test_create_refusals():
         return lib.rst_adamw_create(None if null else t, n, bits, ctypes.byref(s), ctypes.byref(out))
     for change, code in [(dict(null=True), 1), (dict(n=0), 1), (dict(bits=16), 2), (dict(it=None), 1),
                          (dict(param=None), 1), (dict(m=None), 1), (dict(v=None), 1), (dict(bits=8, ms=None), 1),
-                         (dict(bits=8, vs=None), 1), (dict(bits=8, m=p + 4), 1), (dict(count=2 ** 41), 1)]:
+                         (dict(bits=8, vs=None), 1), (dict(bits=8, m=p + 4), 1), (dict(count=2 ** 37), 1),
+                         (dict(count=2 ** 64 - 1), 1)]:
         assert create(**change) == code, (change, lib.rst_last_error())
         assert h.value is None and b"rst_adamw_create" in lib.rst_last_error()
     cfg = L.RstAdamwConfig(1e-3, 0, 0.9, 0.999, 1e-7, 0, 0)

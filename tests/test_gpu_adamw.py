@@ -139,6 +139,46 @@ def test_steps(sizes, bits, dtype, clip):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_a_large_step(bits):
+    """17 M elements: past the caches, the other sizes of a workgroup's share."""
+    sizes = [9, 17000003, 4097]
+    variables, grad, decay = _make(sizes)
+    opt = _adamw(state_bits=bits, global_clipnorm=100.0)
+    opt.build(variables, decay=decay)
+    ref = Reference(opt, variables, decay)
+    for _ in range(2):
+        want = ref.step(ref.read(opt, variables), grad.cpu().numpy())
+        opt.apply_gradients(grad)
+        _compare(want, ref.read(opt, variables), bits)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_offsets_past_32_bits(bits):
+    """One variable of 2^31 + 4099 elements (8.6 GB). The first step from zero states: m / bc1 = g, sqrt(v / bc2) = |g|."""
+    n = 2 ** 31 + 4099
+    p, step = torch.ones(n, device='cuda'), 2 ** 27
+    g = torch.empty(n, dtype=torch.bfloat16, device='cuda')
+    value = lambda lo, hi: ((torch.arange(lo, hi, device='cuda') % 997 - 498).float() * 1e-3).bfloat16()  # noqa: E731
+    for lo in range(0, n, step):
+        g[lo:lo + step] = value(lo, min(lo + step, n))
+    opt = _adamw(state_bits=bits)
+    opt.build([p])
+    opt.apply_gradients(g)
+    for lo in range(0, n, step):
+        gd = value(lo, min(lo + step, n)).double()
+        want = 1.0 - LR * (gd / (gd.abs() + EPS))
+        assert float((p[lo:lo + step].double() - want).abs().max()) <= E + LR * 16 * E
+    assert opt.iterations == 1
+    if bits == 32:
+        assert float((opt.m[-4099:].double() - 0.1 * g[-4099:].double()).abs().max()) <= 0.05 * 4 * E
+    else:
+        last = g[-3:].double()                       # the last block: three elements and zeros
+        got = opt.m[-1].double() * opt.m_scale[-1].double()
+        assert float((got[:3] - 0.1 * last).abs().max()) <= 2.0 ** -4 * 0.1 * float(last.abs().max())
+        assert not got[3:].any() and opt.m.shape[0] == (n + 127) // 128
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("t", [10 ** 3, 10 ** 6, 2 ** 33])
 def test_late_steps(bits, t):
     """Step counts far on: 1 - beta^t from expm1 in 64 bits, the count in 64."""
@@ -355,8 +395,9 @@ def test_trains_a_normalised_layer():
             .reshape(shape) * leaves[1] + leaves[2]
         loss = 0.5 * ((z * torch.sigmoid(z) - target) ** 2).sum()
         loss.backward()
+        loss = float(loss.detach())
         mine = 0.5 * float(((y.double() - target) ** 2).sum())
-        assert abs(mine - float(loss)) < 1e-5 * float(loss) + (t > 1) * 1e-4 * float(loss)
+        assert abs(mine - loss) < 1e-5 * loss + (t > 1) * 1e-4 * loss
         norm = torch.sqrt(sum((l.grad ** 2).sum() for l in leaves))
         c = min(1.0, 5.0 / float(norm))
         for k, leaf in enumerate(leaves):

@@ -24,7 +24,12 @@ SHAPES = [(1, 1, 1, 1, 1),             # one value: variance 0
           (1, 6, 5, 2200, 4),          # several channel blocks, groups across their borders
           (1, 3, 3, 1030, 2), (1, 4, 4, 2048, 1), (1, 2, 3, 1500, 1500),
           (300, 2, 2, 16, 4),          # many small images
-          (1, 300, 301, 2, 1)]         # few channels, many pixels
+          (1, 300, 301, 2, 1),         # few channels, many pixels
+          (300, 50, 42, 4, 2),         # more images than workgroups, two passes each
+          (1, 42, 50, 1025, 5),        # two passes over two channel blocks, a group across their border
+          (1, 42, 50, 1500, 1500),     # more groups than the second pass merges by itself
+          (1, 50, 60, 4400, 11),       # whole vectors in two channel blocks
+          (2, 480, 480, 80, 5)]        # past the caches
 
 
 @pytest.fixture(autouse=True)
@@ -249,22 +254,24 @@ def test_same_bits_every_time_in_graphs_and_on_other_streams():
         assert all(torch.equal(p, q) and torch.equal(p, r) for p, q, r in zip(want, held, eager))
 
 
-def test_in_place_through_the_c_interface():
+@pytest.mark.parametrize("H", [40, 90])              # one launch, two passes
+def test_in_place_through_the_c_interface(H):
     """y may be x, dx may be dy."""
     from realtime_style_transfer_amd import _lib as L
     gn, grad = _op()
     lib = L.load()
-    x, scale, bias, dy = _inputs((2, 40, 50, 24, 3), torch.float32, False)
+    x, scale, bias, dy = _inputs((2, H, 50, 24, 3), torch.float32, False)
+    n = H * 50
     y, mean, rstd = gn(x, scale, bias, 3, activation="relu", return_statistics=True)
     dx, ds, db = grad(x, dy, scale, bias, mean, rstd, 3, "relu")
-    need = max(lib.rst_group_norm_workspace_size(2, 2000, 24, 3), lib.rst_group_norm_backward_workspace_size(2, 2000, 24, 3))
+    need = max(lib.rst_group_norm_workspace_size(2, n, 24, 3), lib.rst_group_norm_backward_workspace_size(2, n, 24, 3))
     ws = torch.empty(need, dtype=torch.uint8, device='cuda')
     d2, s2, b2 = dy.clone(), torch.empty_like(ds), torch.empty_like(db)
-    L.check(lib.rst_group_norm_backward(x.data_ptr(), d2.data_ptr(), 0, 2, 2000, 24, 3, scale.data_ptr(),
+    L.check(lib.rst_group_norm_backward(x.data_ptr(), d2.data_ptr(), 0, 2, n, 24, 3, scale.data_ptr(),
                                         bias.data_ptr(), 0, mean.data_ptr(), rstd.data_ptr(), 1, d2.data_ptr(),
                                         s2.data_ptr(), b2.data_ptr(), ws.data_ptr(), L.stream_ptr()))
     x2 = x.clone()
-    L.check(lib.rst_group_norm(x2.data_ptr(), 0, 2, 2000, 24, 3, scale.data_ptr(), bias.data_ptr(), 0, 1e-5, 1,
+    L.check(lib.rst_group_norm(x2.data_ptr(), 0, 2, n, 24, 3, scale.data_ptr(), bias.data_ptr(), 0, 1e-5, 1,
                                x2.data_ptr(), None, None, ws.data_ptr(), L.stream_ptr()))
     torch.cuda.synchronize()
     assert torch.equal(x2, y) and torch.equal(d2, dx) and torch.equal(s2, ds) and torch.equal(b2, db)
@@ -302,6 +309,54 @@ def test_equals_instance_norm_at_one_channel_per_group():
     ref, z, _, _ = _forward64(x, scale, bias, 24, "relu")
     assert float((b.double() - ref).abs().max()) <= float((a.double() - ref).abs().max()) + 1e-6
     assert float((a - b).abs().max()) < 1e-4           # instance_norm's own bound
+
+
+def test_offsets_past_32_bits():
+    """4.4 G values in one image: elements and bytes beyond 2^32. The statistics by chunks in float64; y, dx at both ends
+    and around the 2^32 border from the returned statistics; the affine's gradients by chunks."""
+    gn, grad = _op()
+    H, W, C, G = 40000, 27500, 4, 2
+    x = torch.empty(1, H, W, C, dtype=torch.bfloat16, device='cuda')
+    for k in range(0, H, 1000):                        # a different spread and mean along the image
+        g = torch.Generator(device='cuda').manual_seed(k)
+        x[0, k:k + 1000] = (torch.randn(1000, W, C, generator=g, device='cuda') * (1 + k / H) + k / H).bfloat16()
+    scale, bias = torch.tensor([1.0, 0.5, -1.0, 2.0], device='cuda'), torch.tensor([0.1, 0.0, 0.3, -0.2], device='cuda')
+    y, mean, rstd = gn(x, scale, bias, G, activation="relu", return_statistics=True)
+    s = torch.zeros(2, G, dtype=torch.float64, device='cuda')
+    for k in range(0, H, 1000):
+        r = x[0, k:k + 1000].double().view(-1, G, 2)
+        s += torch.stack([r.sum((0, 2)), (r * r).sum((0, 2))])
+    m = s[0] / (H * W * 2)
+    _near(mean[0], m, 2 * E * m.abs(), "mean")
+    r = 1 / torch.sqrt(s[1] / (H * W * 2) - m * m + 1e-5)
+    _near(rstd[0], r, 2 * E * r, "rstd")
+    sums = torch.zeros(2, C, dtype=torch.float64, device='cuda')
+    size = torch.zeros(2, C, dtype=torch.float64, device='cuda')
+    wide = lambda t: t[0].double().repeat_interleave(2)  # noqa: E731
+
+    def chunk(rows):
+        xs = x[0, rows].double()
+        h = (xs - wide(mean)) * wide(rstd)
+        dz = (h * scale.double() + bias.double() > 0) * xs      # dy = x below
+        return h, dz
+    for k in range(0, H, 1000):
+        h, dz = chunk(slice(k, k + 1000))
+        sums += torch.stack([(dz * h).sum((0, 1)), dz.sum((0, 1))])
+        size += torch.stack([(dz * h).abs().sum((0, 1)), dz.abs().sum((0, 1))])
+    dx, dscale, dbias = grad(x, x, scale, bias, mean, rstd, G, "relu")
+    _near(dscale, sums[0], 76 * E * size[0], "dscale")
+    _near(dbias, sums[1], 72 * E * size[1], "dbias")
+    n = H * W * 2
+    c1, c2 = ((scale.double() * t).view(G, 2).sum(1).repeat_interleave(2) / n for t in (sums[1], sums[0]))
+    a1, a2 = ((scale.double().abs() * t).view(G, 2).sum(1).repeat_interleave(2) / n for t in (size[1], size[0]))
+    border = 2 ** 32 // (W * C)
+    for rows in (slice(0, 2), slice(border // 2 - 1, border // 2 + 2), slice(border - 1, border + 2), slice(H - 2, H)):
+        h, dz = chunk(rows)
+        z = h * scale.double() + bias.double()
+        _near(y[0, rows], z.clamp(min=0), 2.0 ** -8 * z.abs() + 4 * E * (h.abs() + 1), "y")
+        sc, ri = scale.double(), wide(rstd)
+        want = ri * (sc * dz - c1 - h * c2)
+        _near(dx[0, rows], want, 2.0 ** -8 * want.abs() + ri * 80 * E * ((sc * dz).abs() + a1 + h.abs() * a2), "dx")
 
 
 def test_refusals_on_the_device():
