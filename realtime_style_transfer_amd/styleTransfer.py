@@ -15,6 +15,7 @@ reference initialisers (styleTransfer.py:97,146,190).
 from __future__ import annotations
 
 import ctypes
+import functools
 import logging
 from typing import Dict, List, Optional, Sequence
 
@@ -302,35 +303,41 @@ def instance_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, eps:
 _GN_DTYPES = {torch.float32: _lib.DTYPES["float32"], torch.bfloat16: _lib.DTYPES["bfloat16"]}
 
 
-def _group_norm_check(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, groups: int, activation: str, more):
-    """The shared argument checks of group_norm and group_norm_gradients -> (dtype, activation, per_image)."""
-    if x.dim() != 4:
-        raise ValueError(f"x must be (B,H,W,C), got {tuple(x.shape)}")
-    B, _, _, C = x.shape
-    dtype, act = _GN_DTYPES.get(x.dtype), _lib.ACTIVATIONS.get(activation)
-    if dtype is None:
-        raise ValueError(f"x must be float32 or bfloat16, got {x.dtype}")
+@functools.lru_cache(maxsize=1024)
+def _group_norm_plan(shape, dtype, scale_shape, bias_shape, groups: int, activation: str):
+    """What a group_norm of these sizes is called with, its arguments checked -> (dtype, activation, per_image, B, H W, C,
+    bytes of the forward's and of the backward's workspace)."""
+    if len(shape) != 4:
+        raise ValueError(f"x must be (B,H,W,C), got {tuple(shape)}")
+    B, H, W, C = shape
+    if dtype not in _GN_DTYPES:
+        raise ValueError(f"x must be float32 or bfloat16, got {dtype}")
     if groups < 1 or C < 1 or C % groups != 0:
         raise ValueError(f"{groups} groups do not divide {C} channels")
-    if act is None:
+    if activation not in _lib.ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}; supported: {sorted(_lib.ACTIVATIONS)}")
-    per_image = scale.dim() == 2
-    shape = (B, C) if per_image else (C,)
-    if scale.shape != shape or bias.shape != shape:
-        raise ValueError(f"scale and bias must both be (C,) = ({C},) or (B,C) = ({B},{C}), got {tuple(scale.shape)} and "
-                         f"{tuple(bias.shape)}")
+    per_image = len(scale_shape) == 2
+    if not tuple(scale_shape) == tuple(bias_shape) == ((B, C) if per_image else (C,)):
+        raise ValueError(f"scale and bias must both be (C,) = ({C},) or (B,C) = ({B},{C}), got {tuple(scale_shape)} and "
+                         f"{tuple(bias_shape)}")
+    lib, sizes = _lib.load(), (B, H * W, C, groups)
+    return (_GN_DTYPES[dtype], _lib.ACTIVATIONS[activation], per_image, B, H * W, C,
+            lib.rst_group_norm_workspace_size(*sizes), lib.rst_group_norm_backward_workspace_size(*sizes))
+
+
+def _group_norm_tensors(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, *more) -> int:
+    """The tensors' own checks -> the device's index."""
+    if not x.is_cuda:
+        raise ValueError("librst operates on device tensors; got a CPU tensor")
     if scale.dtype is not torch.float32 or bias.dtype is not torch.float32:
         raise ValueError(f"scale and bias must be float32, got {scale.dtype} and {bias.dtype}")
-    device = x.device
-    if device.type != 'cuda':
-        raise ValueError("librst operates on device tensors; got a CPU tensor")
-    grad = torch.is_grad_enabled()
+    index, grad = x.get_device(), torch.is_grad_enabled()
     for t in (x, scale, bias, *more):
-        if t.device != device:
-            raise ValueError(f"x is on {device}, another tensor on {t.device}")
+        if t.get_device() != index:
+            raise ValueError(f"x is on {x.device}, another tensor on {t.device}")
         if grad and t.requires_grad:
             raise ValueError("group_norm is not recorded by autograd: detach its inputs and use group_norm_gradients")
-    return dtype, act, per_image
+    return index
 
 
 def group_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, groups: int, eps: float = CIN_EPS,
@@ -341,24 +348,22 @@ def group_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, groups:
     x (B,H,W,C) float32 or bfloat16; scale and bias (C,), or (B,C) per image (style parameters), float32; activation
     "linear", "relu", "swish" or "hard_swish". groups == C is ``instance_norm``. Returns y like x; with
     ``return_statistics`` (y, mean, rstd), the statistics (B, groups) float32 that ``group_norm_gradients`` takes."""
-    dtype, act, per_image = _group_norm_check(x, scale, bias, groups, activation, ())
-    B, H, W, C = x.shape
-    index = x.device.index
+    dtype, act, per_image, B, HW, C, need, _ = _group_norm_plan(x.shape, x.dtype, scale.shape, bias.shape, groups,
+                                                                activation)
+    index = _group_norm_tensors(x, scale, bias)
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
             return group_norm(x, scale, bias, groups, eps, activation, return_statistics)
     x, scale, bias = x.contiguous(), scale.contiguous(), bias.contiguous()
-    lib = _lib.load()
     y = torch.empty_like(x)
-    need = lib.rst_group_norm_workspace_size(B, H * W, C, groups)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    ws = scale.new_empty(need // 4) if need else None
     mean = rstd = None
     if return_statistics:
         mean, rstd = scale.new_empty((2, B, groups)).unbind()
-    _lib.check(lib.rst_group_norm(x.data_ptr(), dtype, B, H * W, C, groups, scale.data_ptr(), bias.data_ptr(),
-                                  per_image, eps, act, y.data_ptr(), None if mean is None else mean.data_ptr(),
-                                  None if rstd is None else rstd.data_ptr(), None if ws is None else ws.data_ptr(),
-                                  _lib.device_stream(index)))
+    _lib.check(_lib.load().rst_group_norm(
+        x.data_ptr(), dtype, B, HW, C, groups, scale.data_ptr(), bias.data_ptr(), per_image, eps, act, y.data_ptr(),
+        mean.data_ptr() if return_statistics else None, rstd.data_ptr() if return_statistics else None,
+        ws.data_ptr() if need else None, _lib.device_stream(index)))
     return (y, mean, rstd) if return_statistics else y
 
 
@@ -366,26 +371,24 @@ def group_norm_gradients(x: torch.Tensor, dy: torch.Tensor, scale: torch.Tensor,
                          rstd: torch.Tensor, groups: int, activation: str = "linear"):
     """The gradients of ``group_norm``: from dy = d loss / d y (like x) and the forward's statistics -> (dx like x, dscale,
     dbias shaped as scale; sums over the batch where the affine is shared)."""
-    dtype, act, per_image = _group_norm_check(x, scale, bias, groups, activation, (dy, mean, rstd))
-    B, H, W, C = x.shape
+    dtype, act, per_image, B, HW, C, _, need = _group_norm_plan(x.shape, x.dtype, scale.shape, bias.shape, groups,
+                                                                activation)
+    index = _group_norm_tensors(x, scale, bias, dy, mean, rstd)
     if dy.shape != x.shape or dy.dtype is not x.dtype:
         raise ValueError(f"dy must be like x, {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
     for t in (mean, rstd):
         if t.shape != (B, groups) or t.dtype is not torch.float32:
             raise ValueError(f"mean and rstd must be ({B},{groups}) float32, got {tuple(t.shape)} {t.dtype}")
-    index = x.device.index
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
             return group_norm_gradients(x, dy, scale, bias, mean, rstd, groups, activation)
     x, dy, scale, bias = x.contiguous(), dy.contiguous(), scale.contiguous(), bias.contiguous()
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    lib = _lib.load()
     dx = torch.empty_like(x)
-    dscale, dbias = scale.new_empty((2,) + scale.shape).unbind()
-    need = lib.rst_group_norm_backward_workspace_size(B, H * W, C, groups)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    _lib.check(lib.rst_group_norm_backward(x.data_ptr(), dy.data_ptr(), dtype, B, H * W, C, groups, scale.data_ptr(),
-                                           bias.data_ptr(), per_image, mean.data_ptr(), rstd.data_ptr(), act,
-                                           dx.data_ptr(), dscale.data_ptr(), dbias.data_ptr(),
-                                           None if ws is None else ws.data_ptr(), _lib.device_stream(index)))
+    dscale, dbias = torch.empty_like(scale), torch.empty_like(scale)
+    ws = scale.new_empty(need // 4) if need else None
+    _lib.check(_lib.load().rst_group_norm_backward(
+        x.data_ptr(), dy.data_ptr(), dtype, B, HW, C, groups, scale.data_ptr(), bias.data_ptr(), per_image,
+        mean.data_ptr(), rstd.data_ptr(), act, dx.data_ptr(), dscale.data_ptr(), dbias.data_ptr(),
+        ws.data_ptr() if need else None, _lib.device_stream(index)))
     return dx, dscale, dbias
