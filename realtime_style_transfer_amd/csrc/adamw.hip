@@ -6,7 +6,7 @@
 // One pass over the data: every element's g, p, m, v are read once and p, m, v written once (28 bytes in 32 bits, 16.1
 // with 8-bit states), which is all that bounds it. A workgroup takes one chunk of at most 4096 elements of one variable
 // from a table made once, so a step over hundreds of small variables is one launch. The step count is on the device
-// (a captured step replays as the next one): every workgroup reads t, and the last one to finish writes t + 1.
+// (a captured step replays as the next one): every workgroup reads t, and the last one to have read it writes t + 1.
 //
 // 8-bit states: blocks of 128 elements of one variable with a scale s = max / 448 each, codes in e4m3. m / s rounds to
 // nearest. v / s is rounded up or down at random with the right mean: (1 - b2) of a change is far below half a code, so
@@ -80,7 +80,8 @@ __global__ __launch_bounds__(ADAMW_PTRS) void set_pointers_kernel(AdamwPtrs p, c
     if ((int)threadIdx.x < n) dst[threadIdx.x] = p.p[threadIdx.x];
 }
 
-// Sums of squares over the chunks blockIdx, blockIdx + grid, ...: one partial per workgroup, merged by the step
+// Sums of squares over the chunks blockIdx, blockIdx + grid, ...: one partial per workgroup, merged by the step. 192 MB in
+// 31 us (6.2 TB/s: reading bound), 11 MB in 4.5
 template <bool BF16>
 __global__ __launch_bounds__(NT) void norm_kernel(AdamwArgs a, double* partials) {
     __shared__ double red[4];
@@ -174,6 +175,9 @@ __device__ __forceinline__ void adamw_element(float g, float& p, float& m, float
     p = fmaf(-s.lr, fmaf(s.decay, p, quotient(m, v, s.inv_bc1, s.inv_bc2, s.eps)), p);
 }
 
+// Bound by memory: 48 M elements with bf16 gradients, 1.25 GB, in 214 us (5.8 TB/s; torch's copy of 1 GiB 5.1), 2.7 M
+// elements in 13.6 (their 76 MB stay in the Infinity Cache). Every load of a thread comes before the first use, the step's
+// scalars in between
 template <bool BF16, bool PAST>
 __global__ __launch_bounds__(NT) void adamw32_kernel(AdamwArgs a) {
     __shared__ double red[4];
@@ -387,7 +391,9 @@ __device__ __forceinline__ void step8(Eight& e, const AdamwArgs& a, const AdamwC
     }
 }
 
-// Eight elements per lane and round: a chunk is two rounds
+// Eight elements per lane and round: a chunk is at most two rounds. Bound by memory with about 50 instructions an element
+// beside it: 48 M elements, 774 MB, in 147 us (5.3 TB/s); 61 k elements in 5.0, latency. (Three waves per SIMD: at four
+// the registers spill, 12 M elements 51 and 45 us)
 template <bool BF16, bool PAST>
 __global__ __launch_bounds__(NT, 3) void adamw8_kernel(AdamwArgs a) {
     __shared__ double red[4];

@@ -20,16 +20,11 @@ struct rst_adamw {
     size_t num_blocks = 0;
     bool past = false;                 // the step's data does not stay in the caches
     rst_adamw_state state{};
-    AdamwChunk* d_chunks = nullptr;
-    const void** d_ptrs = nullptr;
-    double* d_partials = nullptr;
+    AdamwChunk* d_chunks = nullptr;    // one allocation: the table, the step counters (zero), partials, gradient pointers
     unsigned* d_tickets = nullptr;
-    ~rst_adamw() {
-        (void)hipFree(d_chunks);
-        (void)hipFree(d_ptrs);
-        (void)hipFree(d_partials);
-        (void)hipFree(d_tickets);
-    }
+    double* d_partials = nullptr;
+    const void** d_ptrs = nullptr;
+    ~rst_adamw() { (void)hipFree(d_chunks); }
 };
 
 namespace {
@@ -135,14 +130,20 @@ int create(const rst_adamw_tensor* tensors, int n, int bits, const rst_adamw_sta
     h->num_blocks = blocks;
     h->state = *state;
     if (chunks.empty()) return RST_OK;
-    const std::vector<unsigned> zeros((1 + (chunks.size() + ADAMW_TICKETS - 1) / ADAMW_TICKETS) * ADAMW_TICKET_STRIDE, 0u);
-    if (hipMalloc(&h->d_chunks, chunks.size() * sizeof(AdamwChunk)) != hipSuccess ||
-        hipMalloc(&h->d_ptrs, n * sizeof(void*)) != hipSuccess ||
-        hipMalloc(&h->d_partials, ADAMW_MAX_PARTIALS * sizeof(double)) != hipSuccess ||
-        hipMalloc(&h->d_tickets, zeros.size() * sizeof(unsigned)) != hipSuccess)
+    const size_t line = ADAMW_TICKET_STRIDE * sizeof(unsigned);
+    const auto lines = [&](size_t bytes) { return (bytes + line - 1) / line * line; };
+    const size_t table = lines(chunks.size() * sizeof(AdamwChunk));
+    const size_t tickets = (1 + (chunks.size() + ADAMW_TICKETS - 1) / ADAMW_TICKETS) * line;
+    const size_t partials = ADAMW_MAX_PARTIALS * sizeof(double);
+    chunks.resize((table + tickets + sizeof(AdamwChunk) - 1) / sizeof(AdamwChunk), AdamwChunk{});   // zeros behind the table
+    char* base = nullptr;
+    if (hipMalloc(&base, chunks.size() * sizeof(AdamwChunk) + line + partials + n * sizeof(void*)) != hipSuccess)
         return set_error(RST_ERR_ALLOC, "rst_adamw_create: device allocation failed");
-    RST_HIP_TRY(hipMemcpy(h->d_chunks, chunks.data(), chunks.size() * sizeof(AdamwChunk), hipMemcpyHostToDevice));
-    RST_HIP_TRY(hipMemcpy(h->d_tickets, zeros.data(), zeros.size() * sizeof(unsigned), hipMemcpyHostToDevice));
+    h->d_chunks = (AdamwChunk*)base;
+    h->d_tickets = (unsigned*)(base + table);
+    h->d_partials = (double*)(base + lines(chunks.size() * sizeof(AdamwChunk)));
+    h->d_ptrs = (const void**)(h->d_partials + ADAMW_MAX_PARTIALS);
+    RST_HIP_TRY(hipMemcpy(base, chunks.data(), chunks.size() * sizeof(AdamwChunk), hipMemcpyHostToDevice));
     return RST_OK;
 }
 

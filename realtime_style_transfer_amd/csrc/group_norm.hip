@@ -77,7 +77,8 @@ __device__ __forceinline__ void add_moments(const Pack<T, V>& v, double* s, doub
     }
 }
 
-// Pass 1: sums of x and x^2 of every (image, group) over a tile
+// Pass 1: sums of x and x^2 of every (image, group) over a tile. Bound by reading x: 59 MB bf16 in 12.1 us (4.9 TB/s),
+// 236 MB f32 in 40.6 (5.8 TB/s; a kernel that only reads: 6.4)
 template <typename T, int V, bool UNI>
 __global__ __launch_bounds__(NT) void gn_stats_kernel(const void* x, Parts parts, Geom g) {
     constexpr int E = UNI ? 1 : V;
@@ -155,7 +156,9 @@ __global__ __launch_bounds__(256) void gn_finalize_kernel(Parts p, float* mean, 
     }
 }
 
-// Pass 2: y = act(a x + c). MERGE: the image's sums are merged here, while the first loads are under way
+// Pass 2: y = act(a x + c). MERGE: the image's sums are merged here, while the first loads are under way. Bound by memory:
+// 59 + 59 MB bf16 in 20.8 us (5.7 TB/s), 236 + 236 MB f32 past the caches in 69 (6.8 TB/s: x comes from the Infinity
+// Cache). 32-bit arithmetic instead of the f64 FMA was no faster (20.9, 68)
 constexpr int MERGE_GROUPS = 1024;
 template <typename T, int V, int ACT, bool MERGE, bool PAST>
 __global__ __launch_bounds__(NT) void gn_apply_kernel(GroupNormArgs a, Parts p, Geom g) {
@@ -211,7 +214,8 @@ __global__ __launch_bounds__(NT) void gn_apply_kernel(GroupNormArgs a, Parts p, 
     });
 }
 
-// One launch: the bundle's values stay in registers between the moments and the output
+// One launch: the bundle's values stay in registers between the moments and the output. Bound by latency: 450 pixels x 96
+// channels 6.1 us, an almost empty image 3.6 in a graph
 template <typename T, int V, bool UNI, int R>
 __global__ __launch_bounds__(NT) void gn_fused_kernel(GroupNormArgs a, Bundle u) {
     constexpr int E = UNI ? 1 : V;
@@ -286,8 +290,8 @@ __global__ __launch_bounds__(NT) void gn_fused_kernel(GroupNormArgs a, Bundle u)
 
 // ---- host ----------------------------------------------------------------------------------------------------------
 
-// The second pass merges where its workgroups read at most this (about 1 us from their L2); past it a launch of its own,
-// about 5 us, is faster
+// The second pass merges where its workgroups read at most this, else a launch of its own does: one image of 28800 pixels
+// x 128 channels, 115 KB 13.6 us (with the launch 13.9, and 3 us more on the host), 230 KB 14.8 (13.8)
 constexpr size_t MERGE_BYTES = 160 << 10;
 
 Geom geometry_of(const GroupNormArgs& a, int V) {

@@ -127,9 +127,7 @@ class AdamW:
                 self.m_scale, self.v_scale = torch.zeros(blocks, device=device), torch.zeros(blocks, device=device)
             self._iterations = torch.zeros(1, dtype=torch.int64, device=device)
             self.global_norm = torch.zeros((), device=device)
-            table = (_lib.RstAdamwTensor * len(counts))()
-            for row, p, c, o, d in zip(table, pointers, counts, offsets, decay):
-                row.param, row.count, row.grad_offset, row.decay = p, c, o, int(bool(d))
+            table = (_lib.RstAdamwTensor * len(counts))(*zip(pointers, counts, offsets, map(bool, decay)))
             scales = (0, 0) if self.state_bits == 32 else (self.m_scale.data_ptr(), self.v_scale.data_ptr())
             state = _lib.RstAdamwState(self.m.data_ptr(), self.v.data_ptr(), *scales, self._iterations.data_ptr(),
                                        self.global_norm.data_ptr())
