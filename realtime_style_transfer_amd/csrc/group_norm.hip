@@ -395,9 +395,11 @@ hipError_t forward(const GroupNormArgs& a, hipStream_t st) {
 
 }  // namespace
 
-// The grids are flat: every (image, channel block, tile) has to be countable in 31 bits at every vector width
+// The grids are flat: every (image, channel block, tile) has to be countable in 31 bits at every vector width. A batch of
+// four pixels of f32 is addressed in 32 bits: fewer than 2^28 channels
 bool group_norm_supported(int batch, long hw, int C, int G) {
     if (batch == 0 || hw == 0) return true;
+    if (C > 1 << 27) return false;
     const Geom g = geometry(batch, hw, C, G, 1, 1, 4, 1);
     return (double)g.B * g.CB * g.tiles < 2147483000.0 && (double)g.B * std::max(g.G, g.C) < 2147483000.0;
 }

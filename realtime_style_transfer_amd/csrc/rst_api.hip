@@ -1132,7 +1132,7 @@ static int group_norm_check(const char* who, int dtype, int batch, int hw, int c
     } else if (activation < RST_ACT_LINEAR || activation > RST_ACT_HARD_SWISH) {
         what = "unknown activation";
     } else if (!group_norm_supported(batch, hw, channels, groups)) {
-        what = "too many workgroups for one launch";
+        what = "too many pixels for one launch, or too many channels";
     }
     return what == nullptr ? RST_OK : fail(code, std::string(who) + ": " + what);
 }

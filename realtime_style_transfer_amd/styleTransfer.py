@@ -310,6 +310,8 @@ def _group_norm_plan(shape, dtype, scale_shape, bias_shape, groups: int, activat
     if len(shape) != 4:
         raise ValueError(f"x must be (B,H,W,C), got {tuple(shape)}")
     B, H, W, C = shape
+    if max(B, H * W, C) > 2 ** 31 - 1:
+        raise ValueError(f"at most 2^31 - 1 images, pixels and channels, got {tuple(shape)}")
     if dtype not in _GN_DTYPES:
         raise ValueError(f"x must be float32 or bfloat16, got {dtype}")
     if groups < 1 or C < 1 or C % groups != 0:
@@ -359,7 +361,8 @@ def group_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, groups:
     ws = scale.new_empty(need // 4) if need else None
     mean = rstd = None
     if return_statistics:
-        mean, rstd = scale.new_empty((2, B, groups)).unbind()
+        # (an empty image has no moments, and nothing is written)
+        mean, rstd = (scale.new_empty((2, B, groups)) if HW else scale.new_full((2, B, groups), float('nan'))).unbind()
     _lib.check(_lib.load().rst_group_norm(
         x.data_ptr(), dtype, B, HW, C, groups, scale.data_ptr(), bias.data_ptr(), per_image, eps, act, y.data_ptr(),
         mean.data_ptr() if return_statistics else None, rstd.data_ptr() if return_statistics else None,

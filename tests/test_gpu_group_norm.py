@@ -379,3 +379,9 @@ def test_refusals_on_the_device():
         grad(x, dy, scale, bias, st[:, :1], st, 2)
     with pytest.raises(ValueError):
         gn(x, scale, bias, 2, eps=-1.0)
+
+
+def test_an_empty_image_has_no_moments():
+    s = torch.ones(8, device='cuda')
+    y, mean, rstd = _op()[0](torch.zeros(2, 3, 0, 8, device='cuda'), s, s, 2, return_statistics=True)
+    assert y.shape == (2, 3, 0, 8) and bool(mean.isnan().all()) and bool(rstd.isnan().all())

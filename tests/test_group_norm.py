@@ -98,3 +98,16 @@ def test_python_refusals_without_a_device():
             group_norm(a['x'], a['scale'], a['bias'], a['groups'], activation=a['activation'])
     with pytest.raises(ValueError):
         group_norm_gradients(x, x, s, s, st, st, 4)
+
+
+def test_sizes_past_the_interface_are_refused():
+    """2^32 pixels are none in 32 bits, and a row of 2^28 channels is past 32 bits of offset."""
+    lib = _lib()
+    keep, x = _buffer()
+    assert _forward(lib, x, channels=2 ** 27 + 8, groups=1, hw=1) == L.RST_ERR_UNSUPPORTED
+    assert lib.rst_group_norm_backward(x, x, F32, 1, 1, 2 ** 28, 2, x, x, 0, x, x, 0, x, x, x, x, None) == \
+        L.RST_ERR_UNSUPPORTED
+    s = torch.ones(1)
+    for shape in ((1, 2 ** 16, 2 ** 16, 1), (2 ** 31, 1, 1, 1)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            group_norm(torch.empty(shape, dtype=torch.bfloat16, device='meta'), s, s, 1)
