@@ -153,7 +153,7 @@ int rst_instance_norm(const float* x, int batch, int hw, int channels, const flo
  * channels, rstd = 1 / sqrt(var + eps), y = act(scale_c (x - mean) rstd + bias_c). x, y, dy and dx are `dtype`
  * (RST_DTYPE_*), everything else f32. scale / bias: (C), or (B, C) with per_image != 0 (style parameters). Any C, any
  * number of groups that divides it, any alignment of the element type; 16-byte alignment with C a multiple of 16 bytes
- * runs on 16-byte loads. y may be x. mean / rstd (B, groups) receive the statistics when not NULL.
+ * runs on 16-byte loads; at most 2^27 channels. y may be x. mean / rstd (B, groups) receive the statistics when not NULL.
  * backward: from dy, x and the forward's mean / rstd: dx (may be dy), dscale and dbias shaped as scale / bias (sums over
  * the batch where they are shared). The same inputs give the same bits (no atomics). batch or hw 0: RST_OK, nothing is
  * written but dscale = dbias = 0. workspace: rst_group_norm(_backward)_workspace_size() bytes (0: may be NULL), aligned to
@@ -344,20 +344,21 @@ int rst_predictor_trainer_set_moving_statistics(rst_predictor_trainer* t, const 
  * One step t for all variables, with c = min(1, global_clipnorm / |g|) over all of them (1 without clipping):
  *   m = beta_1 m + (1 - beta_1) c g;  v = beta_2 v + (1 - beta_2) (c g)^2
  *   p -= learning_rate (m / (1 - beta_1^t) / (sqrt(v / (1 - beta_2^t)) + epsilon) + weight_decay p)
- * weight_decay applies to the variables created with decay != 0. Variables are f32 device memory at any float; gradients
+ * weight_decay applies to the variables created with decay != 0. Variables (not all of them empty) are f32 device memory at any float; gradients
  * (f32 or bf16) come in one bucket, variable k's at element grad_offset of it, or one tensor per variable.
  * State, caller-owned device memory that must outlive the handle:
  *   state_bits 32: m, v f32, the variables' elements one after the other (no gaps).
  *   state_bits 8: m, v e4m3 codes in blocks of 128 elements of one variable, the variables' blocks one after the other
  *     (a variable's last block is filled with zeros), aligned to 8 bytes; m_scale, v_scale one f32 per block. A state
- *     is code * scale, scale = max / 448 (0 where that would be below 2^-126). m / scale rounds to nearest; v / scale rounds up or down at random with the
- *     right mean (bits from a hash of the element, the step and `seed`), never from above zero to zero. The step uses
- *     the m and v before they are rounded.
+ *     is code * scale, scale = max / 448 (0 where that would be below 2^-126). m / scale rounds to nearest; v / scale
+ *     rounds up or down at random with the right mean (bits from a hash of the element, the step and `seed`), never from
+ *     above zero to zero. The step uses the m and v before they are rounded.
  *   iterations: steps taken (t = iterations + 1), moved on by every step on the device: a captured step replays as the
  *     next one. Hyperparameters are captured by value.
  *   global_norm: receives |g| of each step that clips (may be NULL). If |g| is not finite that step changes nothing,
- *     iterations included. Without clipping a NaN spreads as the formula says, with 8 bits an infinity to its block.
- * States start as zeros (iterations 0). One step of a handle at a time: not on two streams at once. */
+ *     iterations included. Without clipping a NaN or an infinity stays with its element, whose moments are NaN then (a
+ *     NaN code, which counts for no scale); a v beyond 448 times f32's largest value saturates.
+ * States start as zeros (iterations 0). A captured step needs the handle for as long as it replays. One step of a handle at a time: not on two streams at once. */
 typedef struct rst_adamw_tensor {
     float* param;
     size_t count;

@@ -272,6 +272,7 @@ __device__ __forceinline__ double max16(double v) {
 }
 
 // A block's scale from its largest value. One that would be subnormal is 0: the block counts as zeros
+constexpr double LARGEST = 448.0 * 3.4028234663852886e38;
 __device__ __forceinline__ float scale_of(double largest) {
     const float s = (float)(largest * (1.0 / 448.0));
     return s < 1.17549435e-38f ? 0.f : s;
@@ -363,13 +364,25 @@ __device__ __forceinline__ void step8(Eight& e, const AdamwArgs& a, const AdamwC
         for (int k = 0; k < 8; ++k)
             if (k < n) store<false, float>(c.param, 4ll * (i + k), e.p[k]);
     }
-    const float new_ms = scale_of(max16(mm)), new_vs = scale_of(max16(vm));
+    float new_ms = scale_of(max16(mm)), new_vs = scale_of(max16(vm));
+    if (!(new_ms < __builtin_inff() && new_vs < __builtin_inff())) {
+        // beyond f32's range: an infinity is left out of its block's scale and becomes a NaN code, a finite v saturates
+        mm = vm = 0.0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (v[k] < __builtin_inf()) v[k] = __builtin_fmin(v[k], LARGEST);
+            mm = __builtin_fmax(mm, fabs(m[k]) < __builtin_inf() ? fabs(m[k]) : 0.0);
+            vm = __builtin_fmax(vm, v[k] < __builtin_inf() ? v[k] : 0.0);
+        }
+        new_ms = scale_of(max16(mm));
+        new_vs = scale_of(max16(vm));
+    }
     const double im = inverse(new_ms), iv = inverse(new_vs);
     const unsigned least = new_vs > 0.f ? 1u : 0u, pair = (unsigned)((unsigned long long)(c.state_at + i) >> 1);
     u32x2 mo, vo;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        // (|m / s| is at most 448 and a rounding: no clamp)
+        // (a finite |m / s| is at most 448 and a rounding: no clamp)
         int w = __builtin_amdgcn_cvt_pk_fp8_f32((float)(m[4 * k] * im), (float)(m[4 * k + 1] * im), 0, false);
         w = __builtin_amdgcn_cvt_pk_fp8_f32((float)(m[4 * k + 2] * im), (float)(m[4 * k + 3] * im), w, true);
         mo[k] = (unsigned)w;
@@ -393,7 +406,7 @@ __device__ __forceinline__ void step8(Eight& e, const AdamwArgs& a, const AdamwC
 
 // Eight elements per lane and round: a chunk is at most two rounds. Bound by memory with about 50 instructions an element
 // beside it: 48 M elements, 774 MB, in 147 us (5.3 TB/s); 61 k elements in 5.0, latency. (Three waves per SIMD: at four
-// the registers spill, 12 M elements 51 and 45 us)
+// the registers spill, 12 M elements 51 us for 48)
 template <bool BF16, bool PAST>
 __global__ __launch_bounds__(NT, 3) void adamw8_kernel(AdamwArgs a) {
     __shared__ double red[4];

@@ -18,6 +18,7 @@ using namespace rst;
 struct rst_adamw {
     int device = 0, bits = 32, num_tensors = 0, num_chunks = 0;
     size_t num_blocks = 0;
+    std::vector<bool> filled;          // per variable: it has elements
     bool past = false;                 // the step's data does not stay in the caches
     rst_adamw_state state{};
     AdamwChunk* d_chunks = nullptr;    // one allocation: the table, the step counters (zero), partials, gradient pointers
@@ -76,7 +77,6 @@ int step_args(rst_adamw* h, const char* who, int dtype, const rst_adamw_config* 
 }
 
 int launch(rst_adamw* h, const AdamwArgs& a, hipStream_t st) {
-    if (h->num_chunks == 0) return RST_OK;
     if (a.num_partials > 0) RST_HIP_TRY(adamw_norm_launch(a, h->d_partials, st));
     RST_HIP_TRY(adamw_step_launch(a, h->bits, h->past, st));
     return RST_OK;
@@ -115,11 +115,13 @@ int create(const rst_adamw_tensor* tensors, int n, int bits, const rst_adamw_sta
             c.decay = t.decay != 0;
             chunks.push_back(c);
         }
+        h->filled.push_back(t.count != 0);
         blocks += (t.count + ADAMW_BLOCK - 1) / ADAMW_BLOCK;
         elements += t.count;
     }
-    if (elements != 0 && (state->m == nullptr || state->v == nullptr ||
-                          (bits == 8 && (state->m_scale == nullptr || state->v_scale == nullptr))))
+    if (elements == 0) return set_error(RST_ERR_INVALID, "rst_adamw_create: no variable has an element");
+    if (state->m == nullptr || state->v == nullptr ||
+        (bits == 8 && (state->m_scale == nullptr || state->v_scale == nullptr)))
         return set_error(RST_ERR_INVALID, "rst_adamw_create: null state");
     if (bits == 8 && (((size_t)state->m | (size_t)state->v) & 7) != 0)
         return set_error(RST_ERR_INVALID, "rst_adamw_create: 8-bit states must be aligned to 8 bytes");
@@ -129,7 +131,6 @@ int create(const rst_adamw_tensor* tensors, int n, int bits, const rst_adamw_sta
     h->num_chunks = (int)chunks.size();
     h->num_blocks = blocks;
     h->state = *state;
-    if (chunks.empty()) return RST_OK;
     const size_t line = ADAMW_TICKET_STRIDE * sizeof(unsigned);
     const auto lines = [&](size_t bytes) { return (bytes + line - 1) / line * line; };
     const size_t table = lines(chunks.size() * sizeof(AdamwChunk));
@@ -179,7 +180,7 @@ void rst_adamw_destroy(rst_adamw* h) { delete h; }
 size_t rst_adamw_num_blocks(const rst_adamw* h) { return h ? h->num_blocks : 0; }
 
 int rst_adamw_step(rst_adamw* h, const void* gradients, int dtype, const rst_adamw_config* config, void* stream) {
-    if (h == nullptr || config == nullptr || (gradients == nullptr && h->num_chunks != 0))
+    if (h == nullptr || config == nullptr || gradients == nullptr)
         return set_error(RST_ERR_INVALID, "rst_adamw_step: null argument");
     AdamwArgs a{};
     const int rc = step_args(h, "rst_adamw_step", dtype, config, a);
@@ -192,17 +193,19 @@ int rst_adamw_step_tensors(rst_adamw* h, const void* const* gradients, int num_t
                            const rst_adamw_config* config, void* stream) {
     if (h == nullptr || config == nullptr || gradients == nullptr || num_tensors != h->num_tensors)
         return set_error(RST_ERR_INVALID, "rst_adamw_step_tensors: null argument, or not one gradient per variable");
+    for (int k = 0; k < num_tensors; ++k)
+        if (gradients[k] == nullptr && h->filled[k])
+            return set_error(RST_ERR_INVALID, "rst_adamw_step_tensors: null gradient");
     AdamwArgs a{};
     const int rc = step_args(h, "rst_adamw_step_tensors", dtype, config, a);
     if (rc != RST_OK) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (h->num_chunks != 0)
-        for (int k = 0; k < num_tensors; k += ADAMW_PTRS) {
-            AdamwPtrs p{};
-            const int n = std::min(ADAMW_PTRS, num_tensors - k);
-            std::copy(gradients + k, gradients + k + n, p.p);
-            RST_HIP_TRY(adamw_set_pointers_launch(p, h->d_ptrs + k, n, st));
-        }
+    for (int k = 0; k < num_tensors; k += ADAMW_PTRS) {
+        AdamwPtrs p{};
+        const int n = std::min(ADAMW_PTRS, num_tensors - k);
+        std::copy(gradients + k, gradients + k + n, p.p);
+        RST_HIP_TRY(adamw_set_pointers_launch(p, h->d_ptrs + k, n, st));
+    }
     return launch(h, a, st);
 }
 

@@ -34,8 +34,8 @@ class AdamW:
     random rounding of 8-bit second moments (reproducible: a hash of element, step and seed).
 
     The hyperparameters are attributes and may be changed between steps. A step captured into a graph keeps those it was
-    captured with, and counts on with every replay (the step count is on the device). One step of an optimizer at a
-    time: not on two streams at once."""
+    captured with, and counts on with every replay (the step count is on the device); keep the optimizer while the graph
+    replays. One step of an optimizer at a time: not on two streams at once."""
 
     def __init__(self, learning_rate: float = 1e-3, weight_decay: float = 4e-3, beta_1: float = 0.9,
                  beta_2: float = 0.999, epsilon: float = 1e-7, global_clipnorm: Optional[float] = None,
@@ -81,7 +81,8 @@ class AdamW:
     # ------------------------------------------------------------------ state
     def build(self, variables: Sequence[torch.Tensor], decay: Optional[Sequence[bool]] = None):
         """Bind the variables (contiguous float32 tensors of one device, updated in place) and make their states, zeros.
-        The gradient bucket holds the variables' gradients one after the other, in this order."""
+        The gradient bucket holds the variables' gradients one after the other, in this order. The memory that a
+        variable has now is what the steps update: one whose ``data`` is replaced later is not followed."""
         variables = list(variables)
         if not variables:
             raise ValueError("no variables")
@@ -94,7 +95,7 @@ class AdamW:
             decay = [v.dim() > 1 for v in variables]
         counts = [v.numel() for v in variables]
         self._build([v.data_ptr() for v in variables], counts, None, decay, device)
-        self._variables = variables
+        self._variables = [v.detach() for v in variables]       # keeps that memory
 
     def _build(self, pointers: Sequence[int], counts: Sequence[int], offsets: Optional[Sequence[int]],
                decay: Sequence[bool], device, owner=None):
@@ -104,6 +105,8 @@ class AdamW:
             raise ValueError("this optimizer already has variables: use one AdamW for each model")
         if len(decay) != len(counts):
             raise ValueError(f"{len(counts)} variables, but decay for {len(decay)}")
+        if not any(counts):
+            raise ValueError("no variable has an element")
         spans = sorted((p, p + 4 * n) for p, n in zip(pointers, counts) if n)
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("two variables share memory")
@@ -135,6 +138,7 @@ class AdamW:
             _lib.check(_lib.load().rst_adamw_create(table, len(counts), self.state_bits, ctypes.byref(state),
                                                     ctypes.byref(h)))
         self._handle = h
+        self._memory = (self.m, self.v, self.m_scale, self.v_scale, self._iterations, self.global_norm)   # the handle's
         self._variables = None
         self._owner = None if owner is None else weakref.ref(owner)
 
@@ -143,6 +147,9 @@ class AdamW:
             raise ValueError("the optimizer has no variables yet: build() it, or compile a training model with it")
         if self._owner is not None and self._owner() is None:
             raise ValueError("the model whose variables this optimizer steps no longer exists")
+
+    def _bound_to(self, owner) -> bool:
+        return self._handle is not None and self._owner is not None and self._owner() is owner
 
     @property
     def iterations(self) -> int:
@@ -174,28 +181,38 @@ class AdamW:
         """Restore the moments (one tensor per variable, any shape of its size). 8-bit states round to nearest, with the
         scale max / 448 of each block."""
         self._require_built()
-        for values, s, scale in ((m, self.m, self.m_scale), (v, self.v, self.v_scale)):
-            values = [torch.as_tensor(t, dtype=torch.float32, device=self.device).reshape(-1) for t in values]
-            if [t.numel() for t in values] != self._counts:
+        rows = []
+        for values in (m, v):
+            rows.append([torch.as_tensor(t, dtype=torch.float32, device=self.device).reshape(-1) for t in values])
+            if [t.numel() for t in rows[-1]] != self._counts:
                 raise ValueError("slots do not match the variables")
+        for values, s, scale in zip(rows, (self.m, self.v), (self.m_scale, self.v_scale)):
             if self.state_bits == 32:
                 s.copy_(torch.cat(values))
                 continue
-            x = torch.cat([torch.nn.functional.pad(t, (0, -t.numel() % BLOCK)) for t in values]).view(-1, BLOCK)
-            scale.copy_((x.double().abs().amax(1) / 448.0).float())
-            y = (x.double() / torch.where(scale > 0, scale, 1.0)[:, None].double()).float().clamp(-448.0, 448.0)
+            x = torch.cat([torch.nn.functional.pad(t, (0, -t.numel() % BLOCK)) for t in values]).view(-1, BLOCK).double()
+            finite = x.isfinite()                              # (the others: a NaN code, and no part in the scale)
+            largest = (torch.where(finite, x.abs(), 0.0).amax(1) / 448.0).float()
+            scale.copy_(torch.where(largest < 2.0 ** -126, 0.0, largest))
+            some = (scale > 0)[:, None]
+            y = torch.where(some, x / torch.where(some, scale[:, None].double(), 1.0), 0.0).float().clamp(-448.0, 448.0)
             if s is self.v:                  # above zero stays above zero: the step divides by its root
-                y = torch.where((x > 0) & (scale > 0)[:, None], y.clamp(min=2.0 ** -9), y)
-            s.copy_(y.to(torch.float8_e4m3fn))
+                y = torch.where((x > 0) & some, y.clamp(min=2.0 ** -9), y)
+            s.copy_(torch.where(finite, y, float('nan')).to(torch.float8_e4m3fn))
 
     # ------------------------------------------------------------------ step
     def apply_gradients(self, gradients: Union[torch.Tensor, Sequence[torch.Tensor]]):
         """One step on the current stream. ``gradients``: the bucket (one contiguous tensor, float32 or bfloat16), or a
         list of one contiguous tensor per variable, all of one dtype."""
         self._require_built()
+        if self._owner is not None:
+            raise ValueError("these variables are a training model's, whose train_step steps them")
+        self._apply(gradients)
+
+    def _apply(self, gradients):
         if torch.cuda.current_device() != self._index:
             with torch.cuda.device(self.device):
-                return self.apply_gradients(gradients)
+                return self._apply(gradients)
         lib, config, stream = _lib.load(), self._check_config(), _lib.device_stream(self._index)
         if isinstance(gradients, torch.Tensor):
             if gradients.numel() != self._bucket_size:

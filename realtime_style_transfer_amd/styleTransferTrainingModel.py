@@ -207,7 +207,7 @@ class StyleTransferTrainingModel:
         """Give an AdamW the trainable weights of both networks: device memory of the trainers, each weight's gradient
         at its place in the bucket (the BN moving statistics between them have none). Kernels decay, biases and norm
         affines do not."""
-        if not isinstance(self.optimizer, AdamW):
+        if not isinstance(self.optimizer, AdamW) or self.optimizer._bound_to(self):
             return
         lib, pr = _lib.load(), self.style_predictor
         groups = [(lib.rst_trainer_weights(self._handle), 0, self._trainable, self._shapes)]
@@ -438,6 +438,10 @@ class StyleTransferTrainingModel:
         keys = {slot: [f"{p}{SLOT_MARK}optimizer/{slot}{VAR_SUFFIX}" for p, _ in paths] for slot in "mv"}
         hyper = {n: f"optimizer/{n}{VAR_SUFFIX}" for n in ("iter",) + _ADAMW_HYPER}
         have = all(k in tensors for ks in keys.values() for k in ks)
+        for ks in keys.values() if have else ():
+            for k, (_, shape) in zip(ks, paths):
+                if tuple(np.shape(tensors[k])) != tuple(shape):
+                    raise ValueError(f"{k} has shape {np.shape(tensors[k])}, the variable {tuple(shape)}")
         used = [k for ks in keys.values() for k in ks] + [k for k in hyper.values() if k in tensors] if have else []
         status = restore_parts(self._checkpoint_parts(), tensors, extra_keys=used)   # validates, then sets weights
         if have:
@@ -562,7 +566,7 @@ class StyleTransferTrainingModel:
     def _apply_adamw(self):
         """One AdamW step of every trainable weight of both networks from the bucket, then the transfer network's
         kernel images follow its weights (the predictor's kernels read theirs in place)."""
-        self.optimizer.apply_gradients(self._grad_bucket)
+        self.optimizer._apply(self._grad_bucket)
         _lib.check(_lib.load().rst_trainer_weights_updated(self._handle, _lib.stream_ptr()))
         self._version += 1
         self.iterations += 1

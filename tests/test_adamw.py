@@ -69,3 +69,14 @@ def test_create_refusals():
     lib.rst_adamw_destroy(None)
     assert not lib.rst_trainer_weights(None) and not lib.rst_predictor_trainer_weights(None)
     assert lib.rst_trainer_weights_updated(None, None) == 1
+
+
+def test_no_elements():
+    lib = _lib()
+    a = np.zeros(64, np.float32)
+    p, h = a.ctypes.data, ctypes.c_void_p()
+    t = (L.RstAdamwTensor * 2)(L.RstAdamwTensor(p, 0, 0, 1), L.RstAdamwTensor(None, 0, 0, 1))
+    s = L.RstAdamwState(p, p, p, p, p, None)
+    assert lib.rst_adamw_create(t, 2, 32, ctypes.byref(s), ctypes.byref(h)) == L.RST_ERR_INVALID and h.value is None
+    with pytest.raises(ValueError, match="no variable has an element"):
+        AdamW()._build([p, p], [0, 0], None, [True, True], 'cuda:0')

@@ -522,3 +522,192 @@ def test_training_model_refusals():
     gc.collect()
     with pytest.raises(ValueError, match="no longer exists"):
         opt.apply_gradients(torch.zeros(size, device='cuda'))
+
+
+def _bytes(opt):
+    return [t.reshape(-1).view(torch.uint8) for t in (opt.m, opt.v, *((opt.m_scale, opt.v_scale) if opt.m_scale is not None else ()))]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_without_clipping_a_bad_gradient_stays_with_its_element(bits):
+    """Against the same steps with zeros in its place: no other element, code or scale differs (a bad moment counts for no
+    scale, as a zero)."""
+    (a, grad, decay), (b, _, _) = _make([300, 5000]), _make([300, 5000])
+    at = torch.tensor([0, 17, 299, 300 + 1234, 300 + 4999], device='cuda')
+    bad = torch.tensor([float('nan'), float('inf'), -float('inf'), float('inf'), float('nan')], device='cuda')
+    x, y = _adamw(state_bits=bits, seed=5), _adamw(state_bits=bits, seed=5)
+    x.build(a, decay=decay)
+    y.build(b, decay=decay)
+    for k in range(3):
+        g = _make([300, 5000], seed=30 + k)[1]
+        x.apply_gradients(g.index_copy(0, at, bad) if k == 0 else g)
+        y.apply_gradients(g.index_fill(0, at, 0.0))
+    other = torch.ones(5300, dtype=torch.bool, device='cuda')
+    other[at] = False
+    for p, q in ((torch.cat(a), torch.cat(b)), *zip(map(torch.cat, x.slots()), map(torch.cat, y.slots()))):
+        assert torch.equal(p[other], q[other])
+    assert bool(torch.cat(a)[at].isnan().all())
+    assert bits == 32 or all(bool(torch.cat(s)[at].isnan().all()) for s in x.slots())
+
+
+def test_a_gradient_past_8_bits_saturates():
+    """(1 - b2) g^2 beyond 448 times the largest f32: v is that number, and nothing is NaN."""
+    variables, grad, decay = _make([256])
+    opt = _adamw(state_bits=8)
+    opt.build(variables, decay=decay)
+    grad[5] = -1e30
+    for _ in range(2):
+        opt.apply_gradients(grad)
+        assert bool(variables[0].isfinite().all()) and bool(opt.m.float().isfinite().all())
+        assert float(opt.v_scale[0]) == torch.finfo(torch.float32).max and float(opt.v.float()[0, 5]) == 448.0
+        assert float(opt.m.float()[0, 5]) == -448.0 and float(opt.v_scale[1]) < 1.0
+
+
+def test_slots_with_bad_values_and_tiny_blocks():
+    variables, grad, decay = _make([256, 128])
+    opt = _adamw(state_bits=8)
+    opt.build(variables, decay=decay)
+    m, v = [torch.randn(256), torch.full((128,), 1e-37)], [torch.rand(256) + 0.1, torch.full((128,), 1e-37)]
+    for t in (m[0], v[0]):
+        t[3], t[200] = float('nan'), float('inf')
+    opt.set_slots(m, v)
+    assert opt.m_scale[2] == 0 and opt.v_scale[2] == 0           # 1e-37 / 448 is below 2^-126: zeros
+    for want, got in zip((m, v), opt.slots()):
+        ok = want[0].isfinite()
+        assert bool(got[0].cpu()[~ok].isnan().all()) and not got[1].any()
+        # a code is within 2^-4 of its value, or half of the smallest, max / 448 2^-10 (v: all of it, 2^-9)
+        off = (got[0].cpu() - want[0]).abs()[ok]
+        assert bool((off <= (2.0 ** -4 + 4 * E) * want[0].abs()[ok] + 5 / 448 * 2.0 ** -9).all())
+    before = _bytes(opt)[0].clone()
+    with pytest.raises(ValueError, match="do not match"):
+        opt.set_slots([t + 1 for t in m], v[:1])
+    assert torch.equal(_bytes(opt)[0], before)                   # nothing is set by halves
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_empty_variables_among_others(bits):
+    import ctypes
+    from realtime_style_transfer_amd import _lib as L
+    sizes = [0, 5, 0, 130, 0]
+    (a, grad, decay), (b, _, _) = _make([5, 130]), _make([5, 130])
+    empty = torch.empty(0, device='cuda')
+    x, y = _adamw(state_bits=bits, global_clipnorm=1.0), _adamw(state_bits=bits, global_clipnorm=1.0)
+    x.build([empty, a[0], empty, a[1], empty], decay=[True, decay[0], True, decay[1], False])
+    y.build(b, decay=decay)
+    x.apply_gradients(grad)
+    x.apply_gradients(list(grad.split(sizes)))
+    for _ in range(2):
+        y.apply_gradients(grad)
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and x.iterations == 2
+    assert [t.numel() for t in x.slots()[0]] == sizes
+    pointers = (ctypes.c_void_p * 5)(None, grad.data_ptr(), None, None, None)      # the fourth one's is missing
+    rc = L.load().rst_adamw_step_tensors(x._handle, pointers, 5, 0, ctypes.byref(x._check_config()), L.stream_ptr())
+    assert rc == L.RST_ERR_INVALID and x.iterations == 2
+
+
+def test_memory_stays_when_its_names_are_given_away():
+    variables, grad, decay = _make([300])
+    opt = _adamw()
+    opt.build(variables, decay=decay)
+    v = variables[0]
+    v.data, opt.m, opt.v = torch.zeros(300, device='cuda'), None, None
+    variables.clear()
+    torch.cuda.empty_cache()
+    opt.apply_gradients(grad)
+    assert not v.any() and opt.iterations == 1
+
+
+def test_a_models_optimizer_steps_with_the_model_alone():
+    from realtime_style_transfer_amd.styleTransferTrainingModel import RMSprop
+    tr, (x, y) = _training_model(_adamw()), _batch()
+    opt = tr.optimizer
+    with pytest.raises(ValueError, match="train_step"):
+        opt.apply_gradients(tr._grad_bucket)               # the kernels' weight images would not follow
+    tr.train_step(x, y)
+    tr.compile(optimizer=RMSprop(learning_rate=1e-3))
+    tr.train_step(x, y)
+    assert opt.iterations == 1 and len(tr.optimizer_slots()) == len(tr.get_weights())
+    tr.compile(optimizer=opt)                              # its own AdamW again, with its moments
+    tr.train_step(x, y)
+    assert opt.iterations == 2 and tr.iterations == 3
+
+
+def test_training_model_without_a_predictor(tmp_path):
+    from realtime_style_transfer_amd.plan import network_plan, synthetic_style_params
+    from realtime_style_transfer_amd.styleTransferTrainingModel import StyleTransferTrainingModel
+    ins, outs, br, bf = (32, 64, 17), (32, 64, 3), 8, 8
+    plan = network_plan(ins, outs, br, bf)
+    x, y = _batch()
+    x = {'content': x['content'],
+         'style_params': torch.from_numpy(synthetic_style_params(2, 1, plan.num_style_params, plan, seed=1)).cuda()}
+    models = [StyleTransferTrainingModel(ins, outs, br, bf, max_batch=2, seed=s, optimizer=_adamw(global_clipnorm=1.0))
+              for s in (2, 3)]
+    models[0].train_step(x, y)
+    models[0].save_weights(str(tmp_path / "ck"))
+    models[1].load_weights(str(tmp_path / "ck")).assert_nontrivial_match()
+    for m in models:
+        m.train_step(x, y)
+    a, b = (np.concatenate([w.ravel() for w in m.get_weights()]) for m in models)
+    assert np.array_equal(a, b) and models[1].optimizer.iterations == 2
+
+
+def test_rmsprop_checkpoint_gives_an_adamw_model_its_weights_alone(tmp_path):
+    from realtime_style_transfer_amd.styleTransferTrainingModel import RMSprop
+    x, y = _batch()
+    a, b = _training_model(RMSprop()), _training_model(_adamw(), seed=5)
+    a.train_step(x, y)
+    a.save_weights(str(tmp_path / "ck"))
+    status = b.load_weights(str(tmp_path / "ck"))
+    with pytest.raises(AssertionError):
+        status.assert_consumed()
+    assert all(np.array_equal(p, q) for p, q in zip(a.get_weights(), b.get_weights()))
+    assert b.optimizer.iterations == 0 and b.optimizer.learning_rate == LR
+    assert not any(t.any() for t in b.optimizer.slots()[0])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_training_step_replays_as_the_next_one(bits):
+    a, b = (_training_model(_adamw(state_bits=bits, global_clipnorm=1.0)) for _ in range(2))
+    x, y = _batch()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a.train_step(x, y)
+        b.train_step(x, y)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        b.train_step(x, y)
+    for k in range(3):
+        a.train_step(x, y)
+        g.replay()
+        torch.cuda.synchronize()
+        wa, wb = (np.concatenate([q.ravel() for q in m.get_weights() + m.style_predictor.get_weights()]) for m in (a, b))
+        assert np.array_equal(wa, wb) and a.optimizer.iterations == b.optimizer.iterations == k + 2
+        assert torch.equal(a.style_losses['loss'], b.style_losses['loss'])
+
+
+def _rank(rank, world, port, tmp):
+    import os
+    import torch.distributed as dist
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    torch.cuda.set_device(0)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        tr = _training_model(_adamw(state_bits=8, global_clipnorm=1.0))
+        x, y = _batch(seed=100 + rank)
+        for _ in range(2):
+            tr.train_step(x, y)
+        w = np.concatenate([q.ravel() for q in tr.get_weights() + tr.style_predictor.get_weights()])
+        np.save(os.path.join(tmp, f"w{rank}.npy"), np.append(w, float(tr.optimizer.global_norm)))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_ranks_stay_identical(tmp_path):
+    import torch.multiprocessing as mp
+    from realtime_style_transfer_amd.frames import free_port
+    mp.spawn(_rank, args=(2, free_port(), str(tmp_path)), nprocs=2, join=True)
+    a, b = (np.load(tmp_path / f"w{r}.npy") for r in range(2))
+    assert np.array_equal(a, b) and np.isfinite(a).all()
