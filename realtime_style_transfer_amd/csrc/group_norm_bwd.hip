@@ -5,7 +5,8 @@
 //   dx = rstd (scale dz - S1 / n - h S2 / n),  S1 = sum_g scale dz, S2 = sum_g scale dz h
 // Two launches, each one pass over x and dy: sums per (tile, channel), then dx, whose workgroups first merge the sums of
 // their image (a third launch where that is too much for each of them); workgroups behind those write the affine's
-// gradients where it is shared by the batch. An image whose groups fit a workgroup's registers takes one launch for dx.
+// gradients where it is shared by the batch. An image whose groups fit a workgroup's registers takes one launch for dx, and
+// a few of them no other for a shared affine's gradients.
 //
 // On which side of a kink z lies is decided exactly: z > k is x > x0 (for scale > 0) with x0 = mean + (k - bias) /
 // (scale rstd) formed in 64 bits and rounded down to f32 once per channel: one f32 comparison per value.
@@ -301,54 +302,66 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(GroupNormArgs a, BwdPa
 }
 
 // One launch: the bundle's x and dy stay in registers between the sums and dx. A shared affine's gradients over several
-// images take the launch of gn_bwd_shared_kernel behind it
+// images: workgroups behind those sum the bundle over all images once more (u.shared), or the launch of
+// gn_bwd_shared_kernel does
 template <typename T, int V, int ACT, int R>
 __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(GroupNormArgs a, double2* sums, Bundle u) {
     __shared__ float2 red[NT * V];
     __shared__ double2 chan[NT];
     __shared__ float2 cg[BUNDLE_GROUPS];
-    const int b = blockIdx.x / u.bundles, first = (blockIdx.x - b * u.bundles) * u.groups;
+    const int image = blockIdx.x / u.bundles, first = (blockIdx.x - image * u.bundles) * u.groups;
+    const bool all = image == u.B;
     const int row = threadIdx.x / u.bv, lane = threadIdx.x - row * u.bv;
     const int vec = first * u.Cg / V + lane, c0 = first * u.Cg;
-    const size_t at = ((size_t)b * u.hw + row) * u.nv + vec, step = (size_t)u.rows * u.nv;
+    const size_t step = (size_t)u.rows * u.nv;
     const bool active = row < u.rows && row < u.hw;
+    int b = all ? 0 : image;
+    size_t at = ((size_t)b * u.hw + row) * u.nv + vec;
     Pack<T, V> x[R], dy[R];
     float s1[V], s2[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
     Channels<ACT, V> k;
-    if (active) {
-        const Pack<T, V>* xs = (const Pack<T, V>*)a.x + at;
-        const Pack<T, V>* ys = (const Pack<T, V>*)a.dy + at;
+    if (active)
+        for (;;) {
+            const Pack<T, V>* xs = (const Pack<T, V>*)a.x + at;
+            const Pack<T, V>* ys = (const Pack<T, V>*)a.dy + at;
 #pragma unroll
-        for (int n = 0; n < R; ++n) {
-            const size_t o = row + n * u.rows < u.hw ? n * step : 0;
-            x[n] = xs[o];
-            dy[n] = ys[o];
-        }
-        k.load(a, b, u.G, u.Cg, vec);
-#pragma unroll
-        for (int n = 0; n < R; ++n)
-            if (row + n * u.rows < u.hw) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) k.add(widen((T)x[n][i]), widen((T)dy[n][i]), i, s1[i], s2[i]);
+            for (int n = 0; n < R; ++n) {
+                const size_t o = row + n * u.rows < u.hw ? n * step : 0;
+                x[n] = xs[o];
+                dy[n] = ys[o];
             }
+            k.load(a, b, u.G, u.Cg, vec);
+            float t2[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) s2[i] *= k.rstd[i];
-    }
+            for (int i = 0; i < V; ++i) t2[i] = 0.f;
+#pragma unroll
+            for (int n = 0; n < R; ++n)
+                if (row + n * u.rows < u.hw) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) k.add(widen((T)x[n][i]), widen((T)dy[n][i]), i, s1[i], t2[i]);
+                }
+#pragma unroll
+            for (int i = 0; i < V; ++i) s2[i] = fmaf(t2[i], k.rstd[i], s2[i]);
+            if (!all || b == u.B - 1) break;
+            ++b;
+            at += (size_t)u.hw * u.nv;
+        }
 #pragma unroll
     for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = make_float2(s1[i], s2[i]);
     __syncthreads();
-    const bool own = a.aff_stride != 0 || u.B == 1;
+    const bool own = all || a.aff_stride != 0 || u.B == 1;
     column_sums(red, u.rows, u.bv * V, u.bv * V, u.threads, [&](int c, double2 s) __attribute__((always_inline)) {
         chan[c] = s;
         if (own) {
             a.dbias[b * a.aff_stride + c0 + c] = (float)s.x;
             a.dscale[b * a.aff_stride + c0 + c] = (float)s.y;
-        } else {
+        } else if (!u.shared) {
             sums[(size_t)b * u.C + c0 + c] = s;
         }
     });
+    if (all) return;
     __syncthreads();
     group_sums(a, b, first, u.groups, u.Cg, u.inv_n, u.threads,
                [&](int c) __attribute__((always_inline)) { return chan[c - c0]; },
@@ -381,6 +394,12 @@ bool fused(int B, long hw, int C, int G, int V, int elem, Bundle& u) {
     return backward_in_one(hw, (size_t)B * hw * C * elem) && bundle(B, hw, C, G, V, MAX_R / 2, NT, u) && u.bv * V <= NT;
 }
 
+// Whether workgroups of the same launch sum a shared affine's gradients over the images, one image after the other, each in
+// R loads: us in a graph so / with the other launch (4 us more on the host): 1024 pixels x 128 channels f32, R = 4,
+// 2 images 7.3 / 8.6, 3 images 11.3 / 10.0; 256 x 256, R = 2, 4 images 6.0 / 6.6, 8 images 10.6 / 7.1; 64 x 512, R = 1,
+// 8 images 6.6 / 6.5
+bool shared_in_one(const Bundle& u) { return u.B > 1 && u.B * u.R <= 8; }
+
 template <typename T, int V, int ACT>
 hipError_t backward_act(const GroupNormArgs& a, hipStream_t st) {
     BwdParts p{};
@@ -389,14 +408,15 @@ hipError_t backward_act(const GroupNormArgs& a, hipStream_t st) {
     const int shared_blocks = (a.C + SHARED_C - 1) / SHARED_C;
     Bundle u;
     if (fused(a.batch, a.hw, a.C, a.G, V, sizeof(T), u)) {
-        const dim3 grid((unsigned)(u.B * u.bundles)), block(u.threads);
+        u.shared = a.aff_stride == 0 && shared_in_one(u);
+        const dim3 grid((unsigned)((u.B + u.shared) * u.bundles)), block(u.threads);
         switch (u.R) {
             case 1: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 1>), grid, block, 0, st, a, p.sums, u); break;
             case 2: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 2>), grid, block, 0, st, a, p.sums, u); break;
             case 4: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 4>), grid, block, 0, st, a, p.sums, u); break;
             default: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 8>), grid, block, 0, st, a, p.sums, u); break;
         }
-        if (a.aff_stride == 0 && a.batch > 1)
+        if (a.aff_stride == 0 && a.batch > 1 && !u.shared)
             hipLaunchKernelGGL(gn_bwd_shared_kernel, dim3((unsigned)shared_blocks), dim3(256), 0, st, p.sums, a.batch, a.C,
                                a.dscale, a.dbias);
         return hipGetLastError();
@@ -447,7 +467,7 @@ size_t group_norm_bwd_workspace_bytes(int batch, long hw, int C, int G) {
     for (size_t a = 1; a <= 4; a *= 2) {
         const int V = vector_width<bf16_t>(2 * a, C, 4);
         Bundle u;
-        if (batch > 1 && fused(batch, hw, C, G, V, 2, u)) n = std::max(n, (size_t)batch * C * sizeof(double2));   // a shared affine's
+        if (batch > 1 && fused(batch, hw, C, G, V, 2, u) && !shared_in_one(u)) n = std::max(n, (size_t)batch * C * sizeof(double2));   // a shared affine's
         if (fused(batch, hw, C, G, V, 4, u)) continue;
         for (int w : {2, 4})
             n = std::max(n, (size_t)batch * C * sizeof(double2) +

@@ -231,6 +231,7 @@ int vector_width(size_t addresses, int n, int v = 16 / (int)sizeof(T)) {
 struct Bundle {
     int B, C, G, Cg, hw;
     int nv, bv, groups, bundles, rows, R, threads;
+    int shared;               // backward: workgroups behind the images' form a shared affine's gradients
     double inv_n;
 };
 constexpr int MAX_R = 16;
@@ -266,7 +267,7 @@ inline bool bundle(int B, long hw, int C, int G, int V, int max_r, int max_threa
     u.R = 1;
     while (u.R * u.rows < hw) u.R *= 2;
     u.inv_n = 1.0 / ((double)hw * Cg);
-    return u.R <= max_r && (double)B * u.bundles < 2147483647.0;
+    return u.R <= max_r && (double)(B + 1) * u.bundles < 2147483647.0;
 }
 
 // When the one-launch form is taken, f32 and bf16 with 32 to 512 channels in groups of 1 to 16 measured: its workgroups

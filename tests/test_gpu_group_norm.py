@@ -385,3 +385,19 @@ def test_an_empty_image_has_no_moments():
     s = torch.ones(8, device='cuda')
     y, mean, rstd = _op()[0](torch.zeros(2, 3, 0, 8, device='cuda'), s, s, 2, return_statistics=True)
     assert y.shape == (2, 3, 0, 8) and bool(mean.isnan().all()) and bool(rstd.isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(2, 37, 53, 24, 6), (3, 5, 5, 32, 32), (8, 4, 4, 64, 8), (9, 4, 4, 64, 8), (4, 16, 16, 256, 32),
+                                   (5, 16, 16, 256, 32), (2, 6, 5, 3, 1), (3, 1, 1, 128, 4), (2, 1, 1, 1, 1), (2, 32, 32, 128, 32)])
+def test_shared_affine_of_few_small_images(shape, dtype):
+    G = shape[-1]
+    for k, act in enumerate(ACTS):
+        x, scale, bias, dy = _inputs(shape, dtype, per_image=False, seed=40 + k)
+        mean, rstd = (t.float() for t in _stats64(x, G, 1e-5))
+        got = _op()[1](x, dy, scale, bias, mean, rstd, G, activation=act)
+        again = _op()[1](x, dy, scale, bias, mean, rstd, G, activation=act)
+        for what, g, h, (want, tol) in zip(("dx", "dscale", "dbias"), got, again,
+                                           _backward64(x, dy, scale, bias, mean, rstd, G, act)):
+            _near(g, want, tol, what)
+            assert torch.equal(g, h)
