@@ -305,11 +305,11 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(GroupNormArgs a, BwdPa
 // images: workgroups behind those sum the bundle over all images once more (u.shared), or the launch of
 // gn_bwd_shared_kernel does
 template <typename T, int V, int ACT, int R>
-__global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(GroupNormArgs a, double2* sums, Bundle u) {
+__global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(GroupNormArgs a, double2* sums, Bundle u, int block0) {
     __shared__ float2 red[NT * V];
     __shared__ double2 chan[NT];
     __shared__ float2 cg[BUNDLE_GROUPS];
-    const int image = blockIdx.x / u.bundles, first = (blockIdx.x - image * u.bundles) * u.groups;
+    const int block = blockIdx.x + block0, image = block / u.bundles, first = (block - image * u.bundles) * u.groups;
     const bool all = image == u.B;
     const int row = threadIdx.x / u.bv, lane = threadIdx.x - row * u.bv;
     const int vec = first * u.Cg / V + lane, c0 = first * u.Cg;
@@ -401,6 +401,17 @@ bool fused(int B, long hw, int C, int G, int V, int elem, Bundle& u) {
 bool shared_in_one(const Bundle& u) { return u.B > 1 && u.B * u.R <= 8; }
 
 template <typename T, int V, int ACT>
+void fused_launch(const GroupNormArgs& a, double2* sums, const Bundle& u, int block0, int blocks, hipStream_t st) {
+    const dim3 grid((unsigned)blocks), block(u.threads);
+    switch (u.R) {
+        case 1: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 1>), grid, block, 0, st, a, sums, u, block0); break;
+        case 2: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 2>), grid, block, 0, st, a, sums, u, block0); break;
+        case 4: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 4>), grid, block, 0, st, a, sums, u, block0); break;
+        default: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 8>), grid, block, 0, st, a, sums, u, block0); break;
+    }
+}
+
+template <typename T, int V, int ACT>
 hipError_t backward_act(const GroupNormArgs& a, hipStream_t st) {
     BwdParts p{};
     p.sums = (double2*)a.workspace;
@@ -409,12 +420,14 @@ hipError_t backward_act(const GroupNormArgs& a, hipStream_t st) {
     Bundle u;
     if (fused(a.batch, a.hw, a.C, a.G, V, sizeof(T), u)) {
         u.shared = a.aff_stride == 0 && shared_in_one(u);
-        const dim3 grid((unsigned)((u.B + u.shared) * u.bundles)), block(u.threads);
-        switch (u.R) {
-            case 1: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 1>), grid, block, 0, st, a, p.sums, u); break;
-            case 2: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 2>), grid, block, 0, st, a, p.sums, u); break;
-            case 4: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 4>), grid, block, 0, st, a, p.sums, u); break;
-            default: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 8>), grid, block, 0, st, a, p.sums, u); break;
+        const int images = u.B * u.bundles;
+        if (!u.shared) {
+            fused_launch<T, V, ACT>(a, p.sums, u, 0, images, st);
+        } else if (a.out == a.dy || a.out == a.x) {      // before dx takes the place of what they read
+            fused_launch<T, V, ACT>(a, p.sums, u, images, u.bundles, st);
+            fused_launch<T, V, ACT>(a, p.sums, u, 0, images, st);
+        } else {
+            fused_launch<T, V, ACT>(a, p.sums, u, 0, images + u.bundles, st);
         }
         if (a.aff_stride == 0 && a.batch > 1 && !u.shared)
             hipLaunchKernelGGL(gn_bwd_shared_kernel, dim3((unsigned)shared_blocks), dim3(256), 0, st, p.sums, a.batch, a.C,

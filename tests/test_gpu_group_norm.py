@@ -401,3 +401,16 @@ def test_shared_affine_of_few_small_images(shape, dtype):
                                            _backward64(x, dy, scale, bias, mean, rstd, G, act)):
             _near(g, want, tol, what)
             assert torch.equal(g, h)
+        for h, g in zip(_backward_in_place(x, dy, scale, bias, mean, rstd, G, k), got):
+            assert torch.equal(g, h)
+
+
+def _backward_in_place(x, dy, scale, bias, mean, rstd, G, act):
+    from realtime_style_transfer_amd import _lib as L
+    lib, (B, H, W, C) = L.load(), x.shape
+    dx, ds, db = dy.clone(), torch.full_like(scale, -1.0), torch.full_like(bias, -1.0)
+    ws = torch.empty(lib.rst_group_norm_backward_workspace_size(B, H * W, C, G) + 16, dtype=torch.uint8, device='cuda')
+    L.check(lib.rst_group_norm_backward(x.data_ptr(), dx.data_ptr(), int(x.dtype is torch.bfloat16), B, H * W, C, G,
+                                        scale.data_ptr(), bias.data_ptr(), 0, mean.data_ptr(), rstd.data_ptr(), act,
+                                        dx.data_ptr(), ds.data_ptr(), db.data_ptr(), ws.data_ptr(), L.stream_ptr()))
+    return dx, ds, db
