@@ -8,8 +8,9 @@
 // gradients where it is shared by the batch. An image whose groups fit a workgroup's registers takes one launch for dx, and
 // a few of them no other for a shared affine's gradients.
 //
-// On which side of a kink z lies is decided exactly: z > k is x > x0 (for scale > 0) with x0 = mean + (k - bias) /
-// (scale rstd) formed in 64 bits and rounded down to f32 once per channel: one f32 comparison per value.
+// On which side of a kink z lies is one f32 comparison per value: z > k is x > x0 (for scale > 0) with x0 = mean + (k - bias) /
+// (scale rstd) formed in 64 bits and rounded down to f32 once per channel, z >= k is x beyond the f32 number below x0. The
+// slopes on the kinks: relu 0 at 0; hard_swish 0 at -3 and 1 at 3, where its forward's branches are.
 #include <hip/hip_runtime.h>
 
 #include "group_norm_device.h"
@@ -36,9 +37,11 @@ struct BwdParts {
     int main_blocks;          // the second pass's workgroups before the shared affine's
 };
 
+// The largest f32 number up to x (UP_TO) or below it
+template <bool UP_TO>
 __device__ __forceinline__ float round_down(double x) {
     const float f = (float)x;
-    if ((double)f <= x || f != f) return f;
+    if ((UP_TO ? (double)f <= x : (double)f < x) || !(f > -__builtin_inff())) return f;      // (-inf and NaN stay)
     const unsigned b = __float_as_uint(f);
     return __uint_as_float(b == 0u || b == 0x80000000u ? 0x80000001u : ((int)b < 0 ? b + 1 : b - 1));
 }
@@ -48,10 +51,13 @@ template <int ACT, int V>
 struct Channels {
     float mean[V], rstd[V], slope[V], bias[V], flip[V], at0[V], at1[V];
 
+    // z > k, or z >= k (INCLUSIVE)
+    template <bool INCLUSIVE>
     __device__ __forceinline__ float threshold(double a, int i, double k) {
-        if (!(a != 0.0)) return (double)bias[i] > k ? -__builtin_inff() : __builtin_inff();
-        const double x0 = (double)mean[i] + (k - (double)bias[i]) / a;
-        return round_down(a > 0.0 ? x0 : -x0);
+        const double b = (double)bias[i];
+        if (!(a != 0.0)) return (INCLUSIVE ? b >= k : b > k) ? -__builtin_inff() : __builtin_inff();
+        const double x0 = (double)mean[i] + (k - b) / a;
+        return round_down<!INCLUSIVE>(a > 0.0 ? x0 : -x0);
     }
     __device__ __forceinline__ void load(const GroupNormArgs& g, int b, int G, int Cg, int vec) {
 #pragma unroll
@@ -65,8 +71,8 @@ struct Channels {
             slope[i] = (float)a;
             if constexpr (ACT == RELU || ACT == HARD_SWISH) {
                 flip[i] = a < 0.0 ? -1.f : 1.f;
-                at0[i] = threshold(a, i, ACT == RELU ? 0.0 : -3.0);
-                if constexpr (ACT == HARD_SWISH) at1[i] = threshold(a, i, 3.0);
+                at0[i] = threshold<false>(a, i, ACT == RELU ? 0.0 : -3.0);
+                if constexpr (ACT == HARD_SWISH) at1[i] = threshold<true>(a, i, 3.0);
             }
         }
     }

@@ -414,3 +414,37 @@ def _backward_in_place(x, dy, scale, bias, mean, rstd, G, act):
                                         scale.data_ptr(), bias.data_ptr(), 0, mean.data_ptr(), rstd.data_ptr(), act,
                                         dx.data_ptr(), ds.data_ptr(), db.data_ptr(), ws.data_ptr(), L.stream_ptr()))
     return dx, ds, db
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(2, 4, 9, 8, 4), (1, 90, 45, 8, 4)])       # one launch, two passes
+@pytest.mark.parametrize("per_image", [False, True])
+def test_the_slope_on_a_kink(shape, dtype, per_image, monkeypatch):
+    """z exactly on a kink and one step of x beside it: hard_swish's slope is 1 from z = 3 on and 0 up to z = -3, relu's 0
+    at 0. Mean 0 and rstd 1 make z = scale x + bias; with scale 0 every pixel lies on the bias. The side of a kink k is the
+    sign of scale x + (bias - k), which 64 bits give exactly: both terms are exact (three-bit scales, small integers) and a
+    rounded sum keeps its sign. (z itself would not do: 3 + 1e-30 rounds to 3.)"""
+    B, H, W, C, G = shape
+    up = 1 + (2.0 ** -7 if dtype is torch.bfloat16 else 2.0 ** -23)
+    down = 1 - (2.0 ** -8 if dtype is torch.bfloat16 else 2.0 ** -24)
+    points = [s * v for s in (1, -1) for v in (0.0, 3.0, 3 * up, 3 * down, 6.0, 1.5, 3.5, 12.0, 1e-30)]
+    x = torch.tensor(points).repeat(-(-B * H * W * C // len(points)))[:B * H * W * C]
+    x = x.view(B, C, H, W).permute(0, 2, 3, 1).contiguous().to(dtype).cuda()
+    scale = torch.tensor([0.0, 0.0, 1.0, -1.0, 1.0, -1.0, 0.5, -2.0]).cuda()
+    bias = torch.tensor([3.0, -3.0, 0.0, 0.0, 3.0, -3.0, 0.0, 3.0]).cuda()
+    if per_image:
+        scale, bias = (t.expand(B, C).contiguous() for t in (scale, bias))
+    dy = _inputs(shape, dtype, False)[3]
+    mean, rstd = torch.zeros(B, G, device='cuda'), torch.ones(B, G, device='cuda')
+
+    def slope(z, act):
+        from_kink = lambda k: x.double().reshape(B, H * W, C) * _wide(scale, B, C) + (_wide(bias, B, C) - k)  # noqa: E731
+        if act == "relu":
+            return (from_kink(0.0) > 0).double(), torch.zeros_like(z)
+        inside = torch.where(from_kink(-3.0) > 0, z / 3 + 0.5, 0.0)
+        return torch.where(from_kink(3.0) >= 0, 1.0, inside), 4 * E * (1 + z.abs())
+    monkeypatch.setitem(globals(), "_slope64", slope)
+    for act in ("relu", "hard_swish"):
+        got = _op()[1](x, dy, scale, bias, mean, rstd, G, activation=act)
+        for what, g, (want, tol) in zip(("dx", "dscale", "dbias"), got, _backward64(x, dy, scale, bias, mean, rstd, G, act)):
+            _near(g, want, tol, f"{act} {what}")
