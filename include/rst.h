@@ -344,8 +344,9 @@ int rst_predictor_trainer_set_moving_statistics(rst_predictor_trainer* t, const 
  * One step t for all variables, with c = min(1, global_clipnorm / |g|) over all of them (1 without clipping):
  *   m = beta_1 m + (1 - beta_1) c g;  v = beta_2 v + (1 - beta_2) (c g)^2
  *   p -= learning_rate (m / (1 - beta_1^t) / (sqrt(v / (1 - beta_2^t)) + epsilon) + weight_decay p)
- * weight_decay applies to the variables created with decay != 0. Variables (not all of them empty) are f32 device memory at any float; gradients
- * (f32 or bf16) come in one bucket, variable k's at element grad_offset of it, or one tensor per variable.
+ * weight_decay applies to the variables created with decay != 0. learning_rate, weight_decay and epsilon are finite in 32
+ * bits, epsilon is at least 2^-126. Variables (not all of them empty) are f32 device memory at any float; gradients (f32 or
+ * bf16) come in one bucket, variable k's at element grad_offset of it, or one tensor per variable.
  * State, caller-owned device memory that must outlive the handle:
  *   state_bits 32: m, v f32, the variables' elements one after the other (no gaps).
  *   state_bits 8: m, v e4m3 codes in blocks of 128 elements of one variable, the variables' blocks one after the other

@@ -33,6 +33,8 @@ namespace {
 // A step that touches more than half of the 256 MB Infinity Cache loads and stores past it (12 M elements, 32-bit states
 // 70 us, through it 80; 6 M 38.9 and 44.4)
 constexpr size_t STREAMING_BYTES = 128u << 20;
+// The kernels take the reciprocal of sqrt(v) + epsilon in f32: below 2^-126 it is infinite, and an element with m = v = 0 a NaN
+constexpr float SMALLEST_EPSILON = 1.17549435e-38f;
 constexpr size_t MAX_ELEMENTS = (size_t)1 << 36;     // 256 GB of variables
 
 int step_args(rst_adamw* h, const char* who, int dtype, const rst_adamw_config* c, AdamwArgs& a) {
@@ -44,9 +46,10 @@ int step_args(rst_adamw* h, const char* who, int dtype, const rst_adamw_config* 
         code = RST_ERR_UNSUPPORTED;
     } else if (!(c->beta_1 >= 0.0 && c->beta_1 < 1.0 && c->beta_2 >= 0.0 && c->beta_2 < 1.0)) {
         what = "beta_1 and beta_2 must lie in [0, 1)";
-    } else if (!std::isfinite(c->learning_rate) || !std::isfinite(c->weight_decay) || !(c->epsilon > 0.0) ||
-               !std::isfinite(c->epsilon) || !(c->global_clipnorm >= 0.0) || !std::isfinite(c->global_clipnorm)) {
-        what = "hyperparameters must be finite, epsilon positive and global_clipnorm not negative";
+    } else if (!std::isfinite((float)c->learning_rate) || !std::isfinite((float)c->weight_decay) ||
+               !((float)c->epsilon >= SMALLEST_EPSILON) || !std::isfinite((float)c->epsilon) ||
+               !(c->global_clipnorm >= 0.0) || !std::isfinite(c->global_clipnorm)) {
+        what = "hyperparameters must be finite in 32 bits, epsilon at least 2^-126 and global_clipnorm not negative";
     } else if (dev != h->device) {
         what = "called on another device than the handle was made on";
     }

@@ -31,7 +31,8 @@ class AdamW:
     """``weight_decay`` applies to the variables ``build`` was given ``decay`` for (by default those with more than one
     dimension: kernels, not biases and norm scales). ``global_clipnorm``: scale the gradients so that their joint norm
     is at most this; a step whose norm is not finite then changes nothing. ``state_bits``: 32 or 8. ``seed``: of the
-    random rounding of 8-bit second moments (reproducible: a hash of element, step and seed).
+    random rounding of 8-bit second moments (reproducible: a hash of element, step and seed). ``learning_rate``,
+    ``weight_decay`` and ``epsilon`` are finite in 32 bits, ``epsilon`` is at least 2^-126.
 
     The hyperparameters are attributes and may be changed between steps. A step captured into a graph keeps those it was
     captured with, and counts on with every replay (the step count is on the device); keep the optimizer while the graph
@@ -71,8 +72,10 @@ class AdamW:
         c.global_clipnorm = 0.0 if clip is None else clip
         if not (0.0 <= c.beta_1 < 1.0 and 0.0 <= c.beta_2 < 1.0):
             raise ValueError(f"beta_1 and beta_2 must lie in [0, 1), got {c.beta_1} and {c.beta_2}")
-        if not (math.isfinite(c.learning_rate) and math.isfinite(c.weight_decay) and 0.0 < c.epsilon < math.inf):
-            raise ValueError("learning_rate, weight_decay and epsilon must be finite, epsilon positive")
+        rate, decay, epsilon = (ctypes.c_float(x).value for x in (c.learning_rate, c.weight_decay, c.epsilon))
+        if not (math.isfinite(rate) and math.isfinite(decay) and 2.0 ** -126 <= epsilon < math.inf):
+            raise ValueError("learning_rate, weight_decay and epsilon must be finite in 32 bits, epsilon at least 2^-126, "
+                             f"got {c.learning_rate}, {c.weight_decay} and {c.epsilon}")
         if not 0.0 <= c.global_clipnorm < math.inf:
             raise ValueError(f"global_clipnorm must be positive and finite, or None, got {clip!r}")
         self._config, self._config_of = c, of

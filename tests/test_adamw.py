@@ -80,3 +80,15 @@ def test_no_elements():
     assert lib.rst_adamw_create(t, 2, 32, ctypes.byref(s), ctypes.byref(h)) == L.RST_ERR_INVALID and h.value is None
     with pytest.raises(ValueError, match="no variable has an element"):
         AdamW()._build([p, p], [0, 0], None, [True, True], 'cuda:0')
+
+
+def test_hyperparameters_that_32_bits_do_not_hold():
+    """The kernels divide by epsilon in 32 bits: below 2^-126 its reciprocal is none there, and 0 / epsilon a NaN."""
+    for bad in (dict(epsilon=1e-50), dict(epsilon=2.0 ** -127), dict(epsilon=1e39), dict(learning_rate=1e39),
+                dict(learning_rate=-1e39), dict(weight_decay=1e39)):
+        with pytest.raises(ValueError, match="32 bits"):
+            AdamW(**bad)
+    opt = AdamW(epsilon=2.0 ** -126, learning_rate=1e38, weight_decay=-1e38)
+    opt.epsilon = 1e-44
+    with pytest.raises(ValueError, match="32 bits"):
+        opt._check_config()

@@ -711,3 +711,25 @@ def test_ranks_stay_identical(tmp_path):
     mp.spawn(_rank, args=(2, free_port(), str(tmp_path)), nprocs=2, join=True)
     a, b = (np.load(tmp_path / f"w{r}.npy") for r in range(2))
     assert np.array_equal(a, b) and np.isfinite(a).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_smallest_epsilon(bits):
+    """2^-126: an element without a gradient stays, the others step by their size; below it the C entry refuses, as for
+    the other hyperparameters past 32 bits."""
+    import ctypes
+    from realtime_style_transfer_amd import _lib as L
+    variables, grad, decay = _make([300, 5])
+    opt = _adamw(state_bits=bits, epsilon=2.0 ** -126, weight_decay=0.0)
+    opt.build(variables, decay=decay)
+    grad[:130] = 0.0
+    before = torch.cat(variables).double()
+    opt.apply_gradients(grad)
+    after = torch.cat(variables).double()
+    assert bool(((after - (before - LR * grad.sign())).abs() <= LR * 16 * E + E * after.abs()).all())
+    lib, kept = L.load(), after.clone()
+    for change in (dict(epsilon=2.0 ** -127), dict(epsilon=1e-50), dict(epsilon=1e39), dict(learning_rate=1e39), dict(weight_decay=-1e39)):
+        c = dict(learning_rate=LR, weight_decay=WD, beta_1=B1, beta_2=B2, epsilon=EPS, global_clipnorm=0.0, seed=0)
+        cfg = L.RstAdamwConfig(*{**c, **change}.values())
+        assert lib.rst_adamw_step(opt._handle, grad.data_ptr(), 0, ctypes.byref(cfg), L.stream_ptr()) == L.RST_ERR_INVALID
+    assert opt.iterations == 1 and torch.equal(torch.cat(variables).double(), kept)
