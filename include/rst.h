@@ -348,7 +348,8 @@ int rst_predictor_trainer_set_moving_statistics(rst_predictor_trainer* t, const 
  * bits, epsilon is at least 2^-126. Variables (not all of them empty) are f32 device memory at any float; gradients (f32 or
  * bf16) come in one bucket, variable k's at element grad_offset of it, or one tensor per variable.
  * State, caller-owned device memory that must outlive the handle:
- *   state_bits 32: m, v f32, the variables' elements one after the other (no gaps).
+ *   state_bits 32: m, v f32, the variables' elements one after the other (no gaps). A v past f32's range (|c g| above
+ *     5.8e20 at beta_2 0.999) is infinite, and its element takes no step but its decay from there on; one below 2^-150 is 0.
  *   state_bits 8: m, v e4m3 codes in blocks of 128 elements of one variable, the variables' blocks one after the other
  *     (a variable's last block is filled with zeros), aligned to 8 bytes; m_scale, v_scale one f32 per block. A state
  *     is code * scale, scale = max / 448 (0 where that would be below 2^-126). m / scale rounds to nearest; v / scale

@@ -733,3 +733,60 @@ def test_the_smallest_epsilon(bits):
         cfg = L.RstAdamwConfig(*{**c, **change}.values())
         assert lib.rst_adamw_step(opt._handle, grad.data_ptr(), 0, ctypes.byref(cfg), L.stream_ptr()) == L.RST_ERR_INVALID
     assert opt.iterations == 1 and torch.equal(torch.cat(variables).double(), kept)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_large_gradients_step_by_the_formula(bits):
+    """v / bc2 past f32's range, and with 8-bit states v itself: the root is still inside. (32-bit states hold g up to
+    sqrt(max / (1 - b2)) = 5.8e20.)"""
+    sizes = [256, 384, 130]
+    variables, grad, decay = _make(sizes)
+    size = torch.logspace(5, 20 if bits == 32 else 37, 770, dtype=torch.float64).float().cuda()
+    grad = grad.sign() * size
+    opt = _adamw(state_bits=bits)
+    opt.build(variables, decay=decay)
+    ref = Reference(opt, variables, decay)
+    for _ in range(3):
+        want = ref.step(ref.read(opt, variables), grad.cpu().numpy())
+        opt.apply_gradients(grad)
+        off = np.abs(ref.read(opt, variables)["p"] - want["p"]) - want["dp"]
+        assert (off <= 0).all(), (float(off.max()), int(off.argmax()))
+
+
+def test_tiny_second_moments():
+    """A v below f32's normal numbers still divides by its root (epsilon 1e-30 beside roots of 1e-20 to 1e-17). One step from
+    given moments with a gradient of 0. v carries half a step of the subnormals, 2^-150, beside its 6 e: half of that,
+    relative to v, is its root's."""
+    n = 512
+    p, g = torch.zeros(n, device='cuda'), torch.zeros(n, device='cuda')
+    opt = _adamw(epsilon=1e-30)
+    opt.build([p])
+    v = torch.logspace(-40, -34, n, dtype=torch.float64).float()
+    m = 0.5 * v.double().sqrt().float() * (1 - 2 * (torch.arange(n) % 2))
+    opt.set_slots([m], [v])
+    opt.iterations = 1000
+    opt.apply_gradients(g)
+    v1 = B2 * v.double()
+    q = B1 * m.double() / (1 - B1 ** 1001) / (torch.sqrt(v1 / (1 - B2 ** 1001)) + 1e-30)
+    tol = LR * q.abs() * (17 * E + 2.0 ** -150 / v1)
+    off = (p.cpu().double() + LR * q).abs() - tol
+    assert bool((off <= 0).all()), (float(off.max()), int(off.argmax()))
+
+
+def test_a_second_moment_past_32_bits():
+    """32-bit states: a v past f32 is infinite, its element decays and takes no step from there on; no other element differs."""
+    (a, grad, decay), (b, _, _) = _make([300, 70]), _make([300, 70])
+    decay = [True, False]
+    x, y = _adamw(), _adamw()
+    x.build(a, decay=decay)
+    y.build(b, decay=decay)
+    at = torch.tensor([11, 299, 300 + 64], device='cuda')
+    before = torch.cat(a)[at].double()
+    for k in range(2):
+        x.apply_gradients(grad.index_copy(0, at, torch.tensor([1e30, -3e38, 1e25], device='cuda')) if k == 0 else grad)
+        y.apply_gradients(grad)
+    other = torch.ones(370, dtype=torch.bool, device='cuda')
+    other[at] = False
+    assert torch.equal(torch.cat(a)[other], torch.cat(b)[other]) and bool(x.v[at].isinf().all())
+    want = before * torch.tensor([(1 - LR * WD) ** 2, (1 - LR * WD) ** 2, 1.0], device='cuda')
+    assert bool(((torch.cat(a)[at].double() - want).abs() <= 8 * E * before.abs()).all())
