@@ -405,7 +405,10 @@ class StyleTransferTrainingModel:
         used, slot_sets = [], []
         if self._handle is not None and isinstance(self.optimizer, AdamW):
             return self._restore_adamw(tensors)
-        if self._handle is not None:
+        # the step count and the rates beside another optimizer's slots are that optimizer's
+        slots = {k.rsplit(f"{SLOT_MARK}optimizer/", 1)[1] for k in tensors if f"{SLOT_MARK}optimizer/" in k}
+        other = bool(slots) and "rms" + VAR_SUFFIX not in slots
+        if self._handle is not None and not other:
             for part, mask, get, set_ in self._slot_groups():
                 keys = [f"{p}{SLOT_MARK}optimizer/rms{VAR_SUFFIX}" if t else None
                         for p, t in zip(part.tree.paths(part.prefix), mask)]
@@ -419,7 +422,7 @@ class StyleTransferTrainingModel:
         for keys, get, set_ in slot_sets:
             set_([np.asarray(tensors[k], np.float32).reshape(c.shape) if k is not None else np.zeros_like(c)
                   for k, c in zip(keys, get())])
-        if self._handle is not None:
+        if self._handle is not None and not other:
             it = tensors.get("optimizer/iter" + VAR_SUFFIX)
             if it is not None:
                 self.iterations = int(it)
