@@ -21,6 +21,7 @@ from typing import Dict, List, Optional, Sequence
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .plan import CIN_EPS, Plan, init_weights, network_plan
@@ -339,6 +340,8 @@ def _group_norm_tensors(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor
             raise ValueError(f"x is on {x.device}, another tensor on {t.device}")
         if grad and t.requires_grad:
             raise ValueError("group_norm is not recorded by autograd: detach its inputs and use group_norm_gradients")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError("group_norm takes no forward-mode tangents: they would be lost")
     return index
 
 

@@ -448,3 +448,21 @@ def test_the_slope_on_a_kink(shape, dtype, per_image, monkeypatch):
         got = _op()[1](x, dy, scale, bias, mean, rstd, G, activation=act)
         for what, g, (want, tol) in zip(("dx", "dscale", "dbias"), got, _backward64(x, dy, scale, bias, mean, rstd, G, act)):
             _near(g, want, tol, f"{act} {what}")
+
+
+def test_forward_mode_gradients_are_refused():
+    """A tangent would be lost silently, as a recorded gradient would."""
+    import torch.autograd.forward_ad as fw
+    gn, grad = _op()
+    x, scale, bias, dy = _inputs((2, 4, 4, 8, 2), torch.float32, False)
+    st = torch.zeros(2, 2, device='cuda')
+    with fw.dual_level():
+        for k, t in enumerate((x, scale, bias)):
+            args = [x, scale, bias]
+            args[k] = fw.make_dual(t, torch.ones_like(t))
+            with pytest.raises(ValueError, match="tangent"):
+                gn(*args, 2)
+        with pytest.raises(ValueError, match="tangent"):
+            grad(x, fw.make_dual(dy, dy), scale, bias, st, st, 2)
+        y = gn(x, scale, bias, 2)                       # none of them has one
+    assert torch.equal(y, gn(x, scale, bias, 2))
