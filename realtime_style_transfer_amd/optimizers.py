@@ -98,7 +98,9 @@ class AdamW:
             decay = [v.dim() > 1 for v in variables]
         counts = [v.numel() for v in variables]
         self._build([v.data_ptr() for v in variables], counts, None, decay, device)
-        self._variables = [v.detach() for v in variables]       # keeps that memory
+        self._variables = [v.detach() for v in variables]       # keeps that memory, and shares its version
+        bases = [v if v._base is None else v._base for v in variables]
+        self._versioned = list({id(b): v for b, v in zip(bases, self._variables)}.values())   # (a buffer's views have one)
 
     def _build(self, pointers: Sequence[int], counts: Sequence[int], offsets: Optional[Sequence[int]],
                decay: Sequence[bool], device, owner=None):
@@ -142,7 +144,7 @@ class AdamW:
                                                     ctypes.byref(h)))
         self._handle = h
         self._memory = (self.m, self.v, self.m_scale, self.v_scale, self._iterations, self.global_norm)   # the handle's
-        self._variables = None
+        self._variables, self._versioned = None, []
         self._owner = None if owner is None else weakref.ref(owner)
 
     def _require_built(self):
@@ -206,11 +208,13 @@ class AdamW:
     # ------------------------------------------------------------------ step
     def apply_gradients(self, gradients: Union[torch.Tensor, Sequence[torch.Tensor]]):
         """One step on the current stream. ``gradients``: the bucket (one contiguous tensor, float32 or bfloat16), or a
-        list of one contiguous tensor per variable, all of one dtype."""
+        list of one contiguous tensor per variable, all of one dtype. Autograd sees the variables change, as in any other
+        operation in place (a captured step: when it is captured, not when it replays)."""
         self._require_built()
         if self._owner is not None:
             raise ValueError("these variables are a training model's, whose train_step steps them")
         self._apply(gradients)
+        torch.autograd.graph.increment_version(self._versioned)
 
     def _apply(self, gradients):
         if torch.cuda.current_device() != self._index:

@@ -812,3 +812,25 @@ def test_adamw_checkpoint_gives_an_rmsprop_model_its_weights_alone(tmp_path):
     c = _training_model(RMSprop())
     c.load_weights(str(tmp_path / "rms")).assert_consumed()
     assert c.iterations == 1 and abs(c.optimizer.learning_rate - 2e-3) < 1e-9 and abs(c.optimizer.rho - 0.8) < 1e-7
+
+
+def test_autograd_sees_a_step():
+    """Variables that a forward has saved are changed by the step: their backward is refused, as after any other change in
+    place."""
+    w = torch.randn(5, 4, device='cuda', requires_grad=True)
+    b = torch.randn(4, device='cuda', requires_grad=True)
+    x = torch.randn(3, 5, device='cuda', requires_grad=True)
+    with torch.inference_mode():
+        frozen = torch.ones(3, device='cuda')            # (has no version)
+    buffer = torch.ones(9, device='cuda')
+    opt = _adamw()
+    opt.build([w, b, frozen, *buffer.split([2, 7])])
+    loss = (x @ w + b).square().sum()
+    versions = [t._version for t in (w, b, buffer)]
+    opt.apply_gradients(torch.ones(36, device='cuda'))
+    assert all(t._version > n for t, n in zip((w, b, buffer), versions))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    (x @ w + b).square().sum().backward()
+    opt.apply_gradients([w.grad, b.grad, torch.zeros(3, device='cuda'), buffer[:2], buffer[2:]])
+    assert opt.iterations == 2
