@@ -387,8 +387,8 @@ class StyleTransferTrainingModel:
                 for (path, shape), value in zip(self._adamw_paths(), values):
                     out[f"{path}{SLOT_MARK}optimizer/{slot}{VAR_SUFFIX}"] = value.cpu().numpy().reshape(shape)
             out["optimizer/iter" + VAR_SUFFIX] = np.array(o.iterations, np.int64)
-            for name in _ADAMW_HYPER:
-                out[f"optimizer/{name}{VAR_SUFFIX}"] = np.array(getattr(o, name), np.float32)
+            for name in _ADAMW_HYPER:        # (64 bits, as the step takes them: a beta_2 next to 1 would round to 1)
+                out[f"optimizer/{name}{VAR_SUFFIX}"] = np.array(getattr(o, name), np.float64)
             return out
         for part, mask, get, _ in self._slot_groups():
             for path, slot, trainable in zip(part.tree.paths(part.prefix), get(), mask):
@@ -455,8 +455,9 @@ class StyleTransferTrainingModel:
                 if self.style_predictor is not None:
                     self.style_predictor.iterations = self.iterations
             for n in _ADAMW_HYPER:
-                if hyper[n] in tensors:     # a float32 variable: its shortest decimal is the number that was set
-                    setattr(o, n, float(str(np.float32(tensors[hyper[n]]))))
+                if hyper[n] in tensors:     # of a float32 variable the shortest decimal is the number that was set
+                    value = np.asarray(tensors[hyper[n]])
+                    setattr(o, n, float(str(np.float32(value))) if value.dtype == np.float32 else float(value))
         return status
 
     def load_weights(self, filepath):

@@ -834,3 +834,22 @@ def test_autograd_sees_a_step():
     (x @ w + b).square().sum().backward()
     opt.apply_gradients([w.grad, b.grad, torch.zeros(3, device='cuda'), buffer[:2], buffer[2:]])
     assert opt.iterations == 2
+
+
+def test_checkpoint_keeps_the_hyperparameters_bits(tmp_path):
+    """In 32 bits a scheduled learning rate would come back rounded, and a beta_2 next to 1 as 1, which no step takes."""
+    x, y = _batch()
+    a = _training_model(_adamw(learning_rate=1e-3 / 3, weight_decay=0.1 / 7, beta_1=0.9 + 1e-9, beta_2=1 - 1e-9))
+    a.train_step(x, y)
+    a.save_weights(str(tmp_path / "ck"))
+    b = _training_model(_adamw(), seed=5)
+    b.load_weights(str(tmp_path / "ck"))
+    names = ('learning_rate', 'weight_decay', 'beta_1', 'beta_2')
+    assert [getattr(a.optimizer, n) for n in names] == [getattr(b.optimizer, n) for n in names]
+    for m in (a, b):
+        m.train_step(x, y)
+    assert all(np.array_equal(p, q) for p, q in zip(a.get_weights(), b.get_weights()))
+    tensors = {k: np.float32(v) if v.dtype == np.float64 else v for k, v in a._checkpoint_tensors().items()}
+    tensors = {k: np.float32(0.999) if k.startswith('optimizer/beta_2') else v for k, v in tensors.items()}
+    b._restore_tensors(tensors)                          # 32-bit variables: their shortest decimal
+    assert b.optimizer.beta_2 == 0.999 and abs(b.optimizer.learning_rate / (1e-3 / 3) - 1) < 2.0 ** -24
