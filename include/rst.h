@@ -153,7 +153,8 @@ int rst_instance_norm(const float* x, int batch, int hw, int channels, const flo
  * channels, rstd = 1 / sqrt(var + eps), y = act(scale_c (x - mean) rstd + bias_c). x, y, dy and dx are `dtype`
  * (RST_DTYPE_*), everything else f32. scale / bias: (C), or (B, C) with per_image != 0 (style parameters). Any C, any
  * number of groups that divides it, any alignment of the element type; 16-byte alignment with C a multiple of 16 bytes
- * runs on 16-byte loads; at most 2^27 channels. y may be x. mean / rstd (B, groups) receive the statistics when not NULL.
+ * runs on 16-byte loads; at most 2^27 channels, batch * channels below 2^31 - 648. y may be x. mean / rstd (B, groups)
+ * receive the statistics when not NULL.
  * backward: from dy, x and the forward's mean / rstd: dx (may be dy), dscale and dbias shaped as scale / bias (sums over
  * the batch where they are shared). The same inputs give the same bits (no atomics). batch or hw 0: RST_OK, nothing is
  * written but dscale = dbias = 0. workspace: rst_group_norm(_backward)_workspace_size() bytes (0: may be NULL), aligned to

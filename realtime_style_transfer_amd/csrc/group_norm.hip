@@ -80,10 +80,10 @@ __device__ __forceinline__ void add_moments(const Pack<T, V>& v, double* s, doub
 // Pass 1: sums of x and x^2 of every (image, group) over a tile. Bound by reading x: 59 MB bf16 in 12.1 us (4.9 TB/s),
 // 236 MB f32 in 40.6 (5.8 TB/s; a kernel that only reads: 6.4)
 template <typename T, int V, bool UNI>
-__global__ __launch_bounds__(NT) void gn_stats_kernel(const void* x, Parts parts, Geom g) {
+__global__ __launch_bounds__(NT) void gn_stats_kernel(const void* x, Parts parts, Geom g, int block0) {
     constexpr int E = UNI ? 1 : V;
     __shared__ double2 red[NT * E];
-    const Place w = place(g, blockIdx.x);
+    const Place w = place(g, blockIdx.x + block0);
     double s[E], q[E];
 #pragma unroll
     for (int k = 0; k < E; ++k) s[k] = q[k] = 0.0;
@@ -142,8 +142,8 @@ struct Merge {
 };
 
 // The merge as a launch of its own, one wave per (image, group)
-__global__ __launch_bounds__(256) void gn_finalize_kernel(Parts p, float* mean, float* rstd, Geom g, float eps) {
-    const long bg = (long)blockIdx.x * 4 + threadIdx.x / 64;
+__global__ __launch_bounds__(256) void gn_finalize_kernel(Parts p, float* mean, float* rstd, Geom g, float eps, int block0) {
+    const long bg = ((long)blockIdx.x + block0) * 4 + threadIdx.x / 64;
     if (bg >= (long)g.B * g.G) return;
     Merge merge;
     merge.load(p, g, (size_t)bg, (int)(bg % g.G), threadIdx.x & 63, 64);
@@ -161,9 +161,9 @@ __global__ __launch_bounds__(256) void gn_finalize_kernel(Parts p, float* mean, 
 // Cache). 32-bit arithmetic instead of the f64 FMA was no faster (20.9, 68)
 constexpr int MERGE_GROUPS = 1024;
 template <typename T, int V, int ACT, bool MERGE, bool PAST>
-__global__ __launch_bounds__(NT) void gn_apply_kernel(GroupNormArgs a, Parts p, Geom g) {
+__global__ __launch_bounds__(NT) void gn_apply_kernel(GroupNormArgs a, Parts p, Geom g, int block0) {
     __shared__ double2 stat[MERGE ? MERGE_GROUPS : 1];
-    const Place w = place(g, blockIdx.x);
+    const Place w = place(g, blockIdx.x + block0);
     const Groups r = groups_of<V>(g, w.cb);
     const int t = team(NT, r.ng);
     int gi = threadIdx.x / t;
@@ -217,11 +217,11 @@ __global__ __launch_bounds__(NT) void gn_apply_kernel(GroupNormArgs a, Parts p, 
 // One launch: the bundle's values stay in registers between the moments and the output. Bound by latency: 450 pixels x 96
 // channels 6.1 us, an almost empty image 3.6 in a graph
 template <typename T, int V, bool UNI, int R>
-__global__ __launch_bounds__(NT) void gn_fused_kernel(GroupNormArgs a, Bundle u) {
+__global__ __launch_bounds__(NT) void gn_fused_kernel(GroupNormArgs a, Bundle u, int block0) {
     constexpr int E = UNI ? 1 : V;
     __shared__ double2 red[(UNI ? NT : NT / 2) * E];
     __shared__ double2 stat[BUNDLE_GROUPS];
-    const int b = blockIdx.x / u.bundles, first = (blockIdx.x - b * u.bundles) * u.groups;   // first group
+    const int block = blockIdx.x + block0, b = block / u.bundles, first = (block - b * u.bundles) * u.groups;   // first group
     const int row = threadIdx.x / u.bv, lane = threadIdx.x - row * u.bv;
     const int vec = first * u.Cg / V + lane;
     const size_t at = ((size_t)b * u.hw + row) * u.nv + vec, step = (size_t)u.rows * u.nv;
@@ -309,32 +309,35 @@ Parts parts_of(const Geom& g, int V) {
 // The widths that the two passes (or the one) can use
 template <int V, typename T, bool UNI>
 hipError_t fused_launch(const GroupNormArgs& a, const Bundle& u, hipStream_t st) {
-    const dim3 grid((unsigned)(u.B * u.bundles)), block(u.threads);
-    switch (u.R) {
-        case 1: hipLaunchKernelGGL((gn_fused_kernel<T, V, UNI, 1>), grid, block, 0, st, a, u); break;
-        case 2: hipLaunchKernelGGL((gn_fused_kernel<T, V, UNI, 2>), grid, block, 0, st, a, u); break;
-        case 4: hipLaunchKernelGGL((gn_fused_kernel<T, V, UNI, 4>), grid, block, 0, st, a, u); break;
-        case 8: hipLaunchKernelGGL((gn_fused_kernel<T, V, UNI, 8>), grid, block, 0, st, a, u); break;
-        default: hipLaunchKernelGGL((gn_fused_kernel<T, V, UNI, 16>), grid, block, 0, st, a, u); break;
-    }
+    in_launches((long)u.B * u.bundles, u.threads, [&](int first, dim3 grid) {
+        const dim3 block(u.threads);
+        switch (u.R) {
+            case 1: hipLaunchKernelGGL((gn_fused_kernel<T, V, UNI, 1>), grid, block, 0, st, a, u, first); break;
+            case 2: hipLaunchKernelGGL((gn_fused_kernel<T, V, UNI, 2>), grid, block, 0, st, a, u, first); break;
+            case 4: hipLaunchKernelGGL((gn_fused_kernel<T, V, UNI, 4>), grid, block, 0, st, a, u, first); break;
+            case 8: hipLaunchKernelGGL((gn_fused_kernel<T, V, UNI, 8>), grid, block, 0, st, a, u, first); break;
+            default: hipLaunchKernelGGL((gn_fused_kernel<T, V, UNI, 16>), grid, block, 0, st, a, u, first); break;
+        }
+    });
     return hipGetLastError();
 }
 
 template <typename T, int V>
 hipError_t apply_launch(const GroupNormArgs& a, const Parts& p, hipStream_t st) {
     const Geom g = geometry_of(a, V);
-    const dim3 grid((unsigned)((long)g.B * g.CB * g.tiles));
-#define GN_APPLY(ACT)                                                                                            \
-    if (p.merge && g.streaming) hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, true, true>), grid, dim3(NT), 0, st, a, p, g); \
-    else if (p.merge) hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, true, false>), grid, dim3(NT), 0, st, a, p, g);  \
-    else if (g.streaming) hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, false, true>), grid, dim3(NT), 0, st, a, p, g); \
-    else hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, false, false>), grid, dim3(NT), 0, st, a, p, g);
-    switch (a.act) {
-        case RELU: GN_APPLY(RELU) break;
-        case SWISH: GN_APPLY(SWISH) break;
-        case HARD_SWISH: GN_APPLY(HARD_SWISH) break;
-        default: GN_APPLY(LINEAR) break;
-    }
+#define GN_APPLY(ACT)                                                                                                         \
+    if (p.merge && g.streaming) hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, true, true>), grid, dim3(NT), 0, st, a, p, g, first); \
+    else if (p.merge) hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, true, false>), grid, dim3(NT), 0, st, a, p, g, first);   \
+    else if (g.streaming) hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, false, true>), grid, dim3(NT), 0, st, a, p, g, first); \
+    else hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, false, false>), grid, dim3(NT), 0, st, a, p, g, first);
+    in_launches((long)g.B * g.CB * g.tiles, NT, [&](int first, dim3 grid) {
+        switch (a.act) {
+            case RELU: GN_APPLY(RELU) break;
+            case SWISH: GN_APPLY(SWISH) break;
+            case HARD_SWISH: GN_APPLY(HARD_SWISH) break;
+            default: GN_APPLY(LINEAR) break;
+        }
+    });
 #undef GN_APPLY
     return hipGetLastError();
 }
@@ -353,10 +356,13 @@ hipError_t stats_launch(const GroupNormArgs& a, hipStream_t st) {
     const Geom ga = geometry_of(a, av);
     const int block_groups = std::min(a.G, (ga.nvb * av - 1) / ga.Cg + 2);
     p.merge = block_groups <= MERGE_GROUPS && (size_t)block_groups * p.slots * g.tiles * sizeof(double2) <= MERGE_BYTES;
-    hipLaunchKernelGGL((gn_stats_kernel<T, V, UNI>), dim3((unsigned)((long)g.B * g.CB * g.tiles)), dim3(NT), 0, st, a.x, p, g);
+    in_launches((long)g.B * g.CB * g.tiles, NT, [&](int first, dim3 grid) {
+        hipLaunchKernelGGL((gn_stats_kernel<T, V, UNI>), grid, dim3(NT), 0, st, a.x, p, g, first);
+    });
     if (!p.merge)
-        hipLaunchKernelGGL(gn_finalize_kernel, dim3((unsigned)(((long)g.B * g.G + 3) / 4)), dim3(256), 0, st, p, a.mean,
-                           a.rstd, g, a.eps);
+        in_launches(((long)g.B * g.G + 3) / 4, 256, [&](int first, dim3 grid) {
+            hipLaunchKernelGGL(gn_finalize_kernel, grid, dim3(256), 0, st, p, a.mean, a.rstd, g, a.eps, first);
+        });
     switch (av) {
         case 8:
             if constexpr (sizeof(T) == 2) return apply_launch<T, 8>(a, p, st);
@@ -395,7 +401,7 @@ hipError_t forward(const GroupNormArgs& a, hipStream_t st) {
 
 }  // namespace
 
-// The grids are flat: every (image, channel block, tile) has to be countable in 31 bits at every vector width. A batch of
+// Workgroups are counted over all launches: every (image, channel block, tile) has to be countable in 31 bits at every vector width. A batch of
 // four pixels of f32 is addressed in 32 bits: fewer than 2^28 channels
 bool group_norm_supported(int batch, long hw, int C, int G) {
     if (batch == 0 || hw == 0) return true;

@@ -129,9 +129,9 @@ __device__ __forceinline__ void column_sums(const float2* red, int rows, int wid
 // Pass 1. 118 + 118 MB bf16 with swish in 44 us (5.3 TB/s), 59 + 59 MB f32 with relu in 23 (5.1 TB/s): bound by reading;
 // swish's 14 instructions a value, two of them at half rate, would take 25 of the 44 by themselves
 template <typename T, int V, int ACT>
-__global__ __launch_bounds__(NT) void gn_bwd_stats_kernel(GroupNormArgs a, BwdParts p, Geom g) {
+__global__ __launch_bounds__(NT) void gn_bwd_stats_kernel(GroupNormArgs a, BwdParts p, Geom g, int block0) {
     __shared__ float2 red[NT * V];
-    const Place w = place(g, blockIdx.x);
+    const Place w = place(g, blockIdx.x + block0);
     float s1[V], s2[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
@@ -159,10 +159,10 @@ __global__ __launch_bounds__(NT) void gn_bwd_stats_kernel(GroupNormArgs a, BwdPa
 
 // The merge as a launch of its own: sums over the tiles, 32 channels by 8 slices per workgroup
 constexpr int FC = 32, FS = 8;
-__global__ __launch_bounds__(FC * FS) void gn_bwd_finalize_kernel(BwdParts p, Geom g) {
+__global__ __launch_bounds__(FC * FS) void gn_bwd_finalize_kernel(BwdParts p, Geom g, int block0) {
     __shared__ double2 red[FC * FS];
     const int cbs = (g.C + FC - 1) / FC;
-    const int b = blockIdx.x / cbs, c = (blockIdx.x - b * cbs) * FC + (threadIdx.x % FC), sl = threadIdx.x / FC;
+    const int block = blockIdx.x + block0, b = block / cbs, c = (block - b * cbs) * FC + (threadIdx.x % FC), sl = threadIdx.x / FC;
     double2 s = make_double2(0.0, 0.0);
     if (c < g.C) {
 #pragma unroll 4
@@ -237,18 +237,19 @@ __device__ __forceinline__ void group_sums(const GroupNormArgs& a, int b, int g0
 // Pass 2. MERGE: the image's sums are merged here, while the first loads are under way (one channel block only). Bound by
 // memory: 236 MB read, 118 MB written in 54 us (6.5 TB/s), 118 and 59 MB in 28.7 (6.2 TB/s)
 template <typename T, int V, int ACT, bool MERGE, bool PAST>
-__global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(GroupNormArgs a, BwdParts p, Geom g) {
+__global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(GroupNormArgs a, BwdParts p, Geom g, int block0) {
     __shared__ double2 chan[MERGE ? MERGE_CHANNELS : 1];
     __shared__ double2 red[NT];
     __shared__ float2 cg[MERGE ? MERGE_CHANNELS : NT * V];     // the block's groups, at most one per channel
-    if ((int)blockIdx.x >= p.main_blocks) {
+    const int block = blockIdx.x + block0;
+    if (block >= p.main_blocks) {
         if constexpr (MERGE)
-            shared_affine(p.part, (long)g.B * g.tiles, g.C, blockIdx.x - p.main_blocks, NT, a.dscale, a.dbias, red);
+            shared_affine(p.part, (long)g.B * g.tiles, g.C, block - p.main_blocks, NT, a.dscale, a.dbias, red);
         else
-            shared_affine(p.sums, g.B, g.C, blockIdx.x - p.main_blocks, NT, a.dscale, a.dbias, red);
+            shared_affine(p.sums, g.B, g.C, block - p.main_blocks, NT, a.dscale, a.dbias, red);
         return;
     }
-    const Place w = place(g, blockIdx.x);
+    const Place w = place(g, block);
     Walk<Pack<T, V>, 2, U<T, ACT>, PAST> walk;
     const void* in[2] = {a.x, a.dy};
     if (w.active) walk.start(in, g, w);
@@ -387,8 +388,8 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(GroupNormArgs a, doubl
         if (row + n * u.rows < u.hw) dx[n * step] = dx_of<T, V, ACT>(k, x[n], dy[n], k1, k2);
 }
 
-__global__ __launch_bounds__(256) void gn_zero_kernel(float* a, float* b, long n) {
-    const long i = blockIdx.x * 256L + threadIdx.x;
+__global__ __launch_bounds__(256) void gn_zero_kernel(float* a, float* b, long n, int block0) {
+    const long i = ((long)blockIdx.x + block0) * 256 + threadIdx.x;
     if (i < n) a[i] = b[i] = 0.f;
 }
 
@@ -408,13 +409,16 @@ bool shared_in_one(const Bundle& u) { return u.B > 1 && u.B * u.R <= 8; }
 
 template <typename T, int V, int ACT>
 void fused_launch(const GroupNormArgs& a, double2* sums, const Bundle& u, int block0, int blocks, hipStream_t st) {
-    const dim3 grid((unsigned)blocks), block(u.threads);
-    switch (u.R) {
-        case 1: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 1>), grid, block, 0, st, a, sums, u, block0); break;
-        case 2: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 2>), grid, block, 0, st, a, sums, u, block0); break;
-        case 4: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 4>), grid, block, 0, st, a, sums, u, block0); break;
-        default: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 8>), grid, block, 0, st, a, sums, u, block0); break;
-    }
+    in_launches(blocks, u.threads, [&](int first, dim3 grid) {
+        const dim3 block(u.threads);
+        first += block0;
+        switch (u.R) {
+            case 1: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 1>), grid, block, 0, st, a, sums, u, first); break;
+            case 2: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 2>), grid, block, 0, st, a, sums, u, first); break;
+            case 4: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 4>), grid, block, 0, st, a, sums, u, first); break;
+            default: hipLaunchKernelGGL((gn_bwd_fused_kernel<T, V, ACT, 8>), grid, block, 0, st, a, sums, u, first); break;
+        }
+    });
 }
 
 template <typename T, int V, int ACT>
@@ -443,18 +447,23 @@ hipError_t backward_act(const GroupNormArgs& a, hipStream_t st) {
     const Geom g = geometry(a.batch, a.hw, a.C, a.G, V, U<T, ACT>, 3 * sizeof(T), THREAD_PX / U<T, ACT>);
     p.merge = g.CB == 1 && a.C <= MERGE_CHANNELS && (size_t)g.tiles * a.C * sizeof(float2) <= MERGE_BYTES;
     p.main_blocks = (int)((long)g.B * g.CB * g.tiles);
-    const dim3 grid((unsigned)p.main_blocks), both((unsigned)(p.main_blocks + (a.aff_stride == 0 ? shared_blocks : 0)));
-    hipLaunchKernelGGL((gn_bwd_stats_kernel<T, V, ACT>), grid, dim3(NT), 0, st, a, p, g);
+    in_launches(p.main_blocks, NT, [&](int first, dim3 grid) {
+        hipLaunchKernelGGL((gn_bwd_stats_kernel<T, V, ACT>), grid, dim3(NT), 0, st, a, p, g, first);
+    });
     if (!p.merge)
-        hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3((unsigned)((long)g.B * ((a.C + FC - 1) / FC))), dim3(FC * FS), 0, st, p, g);
-    if (p.merge && g.streaming)
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, true, true>), both, dim3(NT), 0, st, a, p, g);
-    else if (p.merge)
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, true, false>), both, dim3(NT), 0, st, a, p, g);
-    else if (g.streaming)
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, false, true>), both, dim3(NT), 0, st, a, p, g);
-    else
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, false, false>), both, dim3(NT), 0, st, a, p, g);
+        in_launches((long)g.B * ((a.C + FC - 1) / FC), FC * FS, [&](int first, dim3 grid) {
+            hipLaunchKernelGGL(gn_bwd_finalize_kernel, grid, dim3(FC * FS), 0, st, p, g, first);
+        });
+    in_launches((long)p.main_blocks + (a.aff_stride == 0 ? shared_blocks : 0), NT, [&](int first, dim3 grid) {
+        if (p.merge && g.streaming)
+            hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, true, true>), grid, dim3(NT), 0, st, a, p, g, first);
+        else if (p.merge)
+            hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, true, false>), grid, dim3(NT), 0, st, a, p, g, first);
+        else if (g.streaming)
+            hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, false, true>), grid, dim3(NT), 0, st, a, p, g, first);
+        else
+            hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, false, false>), grid, dim3(NT), 0, st, a, p, g, first);
+    });
     return hipGetLastError();
 }
 
@@ -498,8 +507,9 @@ size_t group_norm_bwd_workspace_bytes(int batch, long hw, int C, int G) {
 hipError_t group_norm_bwd_launch(const GroupNormArgs& a, hipStream_t st) {
     if (a.batch == 0 || a.hw == 0) {      // no pixel: the gradients of the affine are empty sums
         const long n = (long)a.C * (a.aff_stride != 0 ? a.batch : 1);
-        if (n > 0)
-            hipLaunchKernelGGL(gn_zero_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a.dscale, a.dbias, n);
+        in_launches((n + 255) / 256, 256, [&](int first, dim3 grid) {
+            hipLaunchKernelGGL(gn_zero_kernel, grid, dim3(256), 0, st, a.dscale, a.dbias, n, first);
+        });
         return hipGetLastError();
     }
     return a.bf16 ? backward<bf16_t>(a, st) : backward<float>(a, st);

@@ -74,6 +74,13 @@ struct Place {
     bool active;
 };
 
+// HIP launches fewer than 2^32 threads: more workgroups (many tiny images) go in several launches, launch(first workgroup, grid)
+template <typename F>
+void in_launches(long blocks, int threads, F&& launch) {
+    const long most = 0xFFFFFFFFL / threads;
+    for (long first = 0; first < blocks; first += most) launch((int)first, dim3((unsigned)std::min(most, blocks - first)));
+}
+
 __device__ __forceinline__ Place place(const Geom& g, int block) {
     Place w;
     const int per = g.CB * g.tiles;

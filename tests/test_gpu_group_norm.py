@@ -466,3 +466,30 @@ def test_forward_mode_gradients_are_refused():
             grad(x, fw.make_dual(dy, dy), scale, bias, st, st, 2)
         y = gn(x, scale, bias, 2)                       # none of them has one
     assert torch.equal(y, gn(x, scale, bias, 2))
+
+
+def _device_inputs(shape, per_image, seed):
+    B, H, W, C, G = shape
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device='cuda')  # noqa: E731
+    aff = (B, C) if per_image else (C,)
+    return r(B, H, W, C), 1 + 0.3 * r(*aff), 0.5 * r(*aff), r(B, H, W, C)
+
+
+# 2^32 threads and more: each kernel's workgroups take several launches
+@pytest.mark.parametrize("shape", [(2 ** 22 + 3, 1, 1, 8, 2),          # the two passes of 1024 threads
+                                   (61100, 1, 1, 1100, 1100)])         # the merge of 67 M groups, 4 of them in 256 threads
+def test_more_workgroups_than_a_launch_takes(shape):
+    x, scale, bias, _ = _device_inputs(shape, False, 1)
+    _check_forward(x, scale, bias, shape[-1], "swish")
+
+
+@pytest.mark.parametrize("shape, per_image", [((2 ** 22 + 3, 2, 3, 8, 2), False), ((2 ** 22 + 3, 2, 3, 8, 2), True),
+                                              ((2 ** 24 + 5, 1, 1, 4, 1), True)])    # the one-launch form, 256 threads
+def test_more_workgroups_than_a_launch_takes_backward(shape, per_image):
+    x, scale, bias, dy = _device_inputs(shape, per_image, 2)
+    mean, rstd = (t.float() for t in _stats64(x, shape[-1], 1e-5))
+    got = _op()[1](x, dy, scale, bias, mean, rstd, shape[-1], activation="relu")
+    for what, g, (want, tol) in zip(("dx", "dscale", "dbias"), got,
+                                    _backward64(x, dy, scale, bias, mean, rstd, shape[-1], "relu")):
+        _near(g, want, tol, what)
