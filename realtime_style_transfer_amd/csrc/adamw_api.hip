@@ -33,6 +33,7 @@ namespace {
 // A step that touches more than half of the 256 MB Infinity Cache loads and stores past it (12 M elements, 32-bit states
 // 70 us, through it 80; 6 M 38.9 and 44.4)
 constexpr size_t STREAMING_BYTES = 128u << 20;
+constexpr size_t MAX_CHUNKS = 0xFFFFFFFFu / 256;     // HIP launches fewer than 2^32 threads, 256 of them a chunk's
 // The kernels take the reciprocal of sqrt(v) + epsilon in f32: below 2^-126 it is infinite, and an element with m = v = 0 a NaN
 constexpr float SMALLEST_EPSILON = 1.17549435e-38f;
 constexpr size_t MAX_ELEMENTS = (size_t)1 << 36;     // 256 GB of variables
@@ -102,8 +103,16 @@ int create(const rst_adamw_tensor* tensors, int n, int bits, const rst_adamw_sta
             return set_error(RST_ERR_INVALID, "rst_adamw_create: more elements than a device holds");
     }
     h->past = total * (bits == 8 ? 14 : 26) > STREAMING_BYTES;
-    const size_t chunk = chunk_size(total, bits, h->past);
-    chunks.reserve(total / chunk + n);
+    const auto count = [&](size_t chunk) {
+        size_t num = 0;
+        for (int k = 0; k < n; ++k) num += (tensors[k].count + chunk - 1) / chunk;
+        return num;
+    };
+    size_t chunk = chunk_size(total, bits, h->past);
+    if (count(chunk) > MAX_CHUNKS) chunk = ADAMW_CHUNK;
+    if (count(chunk) > MAX_CHUNKS)
+        return set_error(RST_ERR_UNSUPPORTED, "rst_adamw_create: more workgroups than one launch takes");
+    chunks.reserve(count(chunk));
     for (int k = 0; k < n; ++k) {
         const rst_adamw_tensor& t = tensors[k];
         if (t.count != 0 && t.param == nullptr) return set_error(RST_ERR_INVALID, "rst_adamw_create: null variable");

@@ -92,3 +92,15 @@ def test_hyperparameters_that_32_bits_do_not_hold():
     opt.epsilon = 1e-44
     with pytest.raises(ValueError, match="32 bits"):
         opt._check_config()
+
+
+def test_more_workgroups_than_a_launch_takes_are_refused():
+    """HIP launches fewer than 2^32 threads: 2^24 chunks of 256. A variable's chunk is 4096 elements at most."""
+    lib = _lib()
+    a = np.zeros(64, np.float32)
+    p, h = a.ctypes.data, ctypes.c_void_p()
+    s = L.RstAdamwState(p, p, p, p, p, None)
+    half = (L.RstAdamwTensor * 2)(L.RstAdamwTensor(p, 2 ** 35, 0, 1), L.RstAdamwTensor(p, 2 ** 35, 2 ** 35, 1))
+    for bits in (8, 32):
+        assert lib.rst_adamw_create(half, 2, bits, ctypes.byref(s), ctypes.byref(h)) == L.RST_ERR_UNSUPPORTED
+        assert h.value is None and b"one launch" in lib.rst_last_error()
