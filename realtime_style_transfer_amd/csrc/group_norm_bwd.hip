@@ -89,15 +89,15 @@ struct Channels {
         }
         return dy;
     }
-    // a value's share of the sums of dz and dz d (the latter times rstd is that of dz h)
+    // a value's share of the sums of dz and dz h (dz d, to be multiplied by rstd later, can pass f32)
     __device__ __forceinline__ void add(float x, float dy, int i, float& s1, float& s2) const {
         const float d = x - mean[i], g = dz(x, d, dy, i);
         s1 += g;
-        s2 = fmaf(g, d, s2);
+        s2 = fmaf(g, d * rstd[i], s2);
     }
 };
 
-// dx = slope dz - k1 - d k2 with k1 = rstd S1 / n, k2 = rstd^2 S2 / n
+// dx = slope dz - k1 - h k2 with k1 = rstd S1 / n, k2 = rstd S2 / n
 template <typename T, int V, int ACT>
 __device__ __forceinline__ Pack<T, V> dx_of(const Channels<ACT, V>& k, const Pack<T, V>& xs, const Pack<T, V>& dys,
                                             const float (&k1)[V], const float (&k2)[V]) {
@@ -105,7 +105,7 @@ __device__ __forceinline__ Pack<T, V> dx_of(const Channels<ACT, V>& k, const Pac
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const float x = widen((T)xs[i]), d = x - k.mean[i];
-        o[i] = narrow<T>(fmaf(k.slope[i], k.dz(x, d, widen((T)dys[i]), i), -fmaf(d, k2[i], k1[i])));
+        o[i] = narrow<T>(fmaf(k.slope[i], k.dz(x, d, widen((T)dys[i]), i), -fmaf(d * k.rstd[i], k2[i], k1[i])));
     }
     return o;
 }
@@ -145,8 +145,6 @@ __global__ __launch_bounds__(NT) void gn_bwd_stats_kernel(GroupNormArgs a, BwdPa
 #pragma unroll
             for (int i = 0; i < V; ++i) k.add(widen((T)v[0][i]), widen((T)v[1][i]), i, s1[i], s2[i]);
         });
-#pragma unroll
-        for (int i = 0; i < V; ++i) s2[i] *= k.rstd[i];
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = make_float2(s1[i], s2[i]);
@@ -301,7 +299,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(GroupNormArgs a, BwdPa
     for (int i = 0; i < V; ++i) {
         const float2 v = cg[(w.vec * V + i) / g.Cg - g0];
         k1[i] = k.rstd[i] * v.x;
-        k2[i] = k.rstd[i] * (k.rstd[i] * v.y);
+        k2[i] = k.rstd[i] * v.y;
     }
     walk.run([&](const Pack<T, V>(&v)[2], size_t at, unsigned off) __attribute__((always_inline)) {
         put<PAST>((char*)a.out, at, off, dx_of<T, V, ACT>(k, v[0], v[1], k1, k2));
@@ -340,17 +338,12 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(GroupNormArgs a, doubl
                 dy[n] = ys[o];
             }
             k.load(a, b, u.G, u.Cg, vec);
-            float t2[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) t2[i] = 0.f;
 #pragma unroll
             for (int n = 0; n < R; ++n)
                 if (row + n * u.rows < u.hw) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) k.add(widen((T)x[n][i]), widen((T)dy[n][i]), i, s1[i], t2[i]);
+                    for (int i = 0; i < V; ++i) k.add(widen((T)x[n][i]), widen((T)dy[n][i]), i, s1[i], s2[i]);
                 }
-#pragma unroll
-            for (int i = 0; i < V; ++i) s2[i] = fmaf(t2[i], k.rstd[i], s2[i]);
             if (!all || b == u.B - 1) break;
             ++b;
             at += (size_t)u.hw * u.nv;
@@ -380,7 +373,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(GroupNormArgs a, doubl
     for (int i = 0; i < V; ++i) {
         const float2 v = cg[(vec * V + i) / u.Cg - first];
         k1[i] = k.rstd[i] * v.x;
-        k2[i] = k.rstd[i] * (k.rstd[i] * v.y);
+        k2[i] = k.rstd[i] * v.y;
     }
     Pack<T, V>* dx = (Pack<T, V>*)a.out + at;
 #pragma unroll

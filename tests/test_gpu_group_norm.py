@@ -493,3 +493,17 @@ def test_more_workgroups_than_a_launch_takes_backward(shape, per_image):
     for what, g, (want, tol) in zip(("dx", "dscale", "dbias"), got,
                                     _backward64(x, dy, scale, bias, mean, rstd, shape[-1], "relu")):
         _near(g, want, tol, what)
+
+
+@pytest.mark.parametrize("size", [1e25, 1e-25])
+@pytest.mark.parametrize("shape", [(2, 7, 9, 24, 3), (1, 90, 45, 8, 4)])       # one launch, two passes
+def test_gradients_of_activations_far_from_one(shape, size):
+    """rstd^2 and dy (x - mean) are past f32 where dx, dscale and dbias are not."""
+    G = shape[-1]
+    for act in ACTS:
+        x, scale, bias, dy = _inputs(shape, torch.float32, True, seed=50)
+        x, dy = x * size, dy * size ** 0.6        # (dx ~ dy / size)
+        mean, rstd = (t.float() for t in _stats64(x, G, 0.0))
+        got = _op()[1](x, dy, scale, bias, mean, rstd, G, activation=act)
+        for what, g, (want, tol) in zip(("dx", "dscale", "dbias"), got, _backward64(x, dy, scale, bias, mean, rstd, G, act)):
+            _near(g, want, tol, f"{act} {what}")
