@@ -170,14 +170,15 @@ class AdamW:
         self._iterations.fill_(int(value))
 
     def slots(self) -> Tuple[List[torch.Tensor], List[torch.Tensor]]:
-        """The moments m and v of every variable as flat float32 tensors (8-bit states: the values they stand for)."""
+        """The moments m and v of every variable as flat float32 tensors (8-bit states: the values they stand for, at most
+        float32's largest number)."""
         self._require_built()
-        out = []
+        out, top = [], torch.finfo(torch.float32).max
         for s, scale in ((self.m, self.m_scale), (self.v, self.v_scale)):
             if self.state_bits == 32:
                 out.append([t.clone() for t in s.split(self._counts)])
             else:
-                flat = (s.float() * scale[:, None]).reshape(-1)
+                flat = (s.float() * scale[:, None]).clamp_(-top, top).reshape(-1)      # (a NaN stays)
                 rows = [BLOCK * ((c + BLOCK - 1) // BLOCK) for c in self._counts]
                 out.append([t[:c].clone() for t, c in zip(flat.split(rows), self._counts)])
         return out[0], out[1]

@@ -853,3 +853,22 @@ def test_checkpoint_keeps_the_hyperparameters_bits(tmp_path):
     tensors = {k: np.float32(0.999) if k.startswith('optimizer/beta_2') else v for k, v in tensors.items()}
     b._restore_tensors(tensors)                          # 32-bit variables: their shortest decimal
     assert b.optimizer.beta_2 == 0.999 and abs(b.optimizer.learning_rate / (1e-3 / 3) - 1) < 2.0 ** -24
+
+
+def test_slots_of_saturated_states_are_finite():
+    """448 times a scale can be past f32: a slot is its largest number then, and restored it is no infinity."""
+    (variables, grad, decay), top = _make([256]), torch.finfo(torch.float32).max
+    opt, other = _adamw(state_bits=8), _adamw(state_bits=8)
+    opt.build(variables, decay=decay)
+    other.build([v.clone() for v in variables], decay=decay)
+    grad[5], grad[9], grad[200] = -1e30, 1e25, float('nan')
+    opt.apply_gradients(grad)
+    m, v = opt.slots()
+    assert float(v[0][5]) == float(v[0][9]) == top and bool(v[0][200].isnan())
+    other.set_slots(m, v)
+    other.iterations = 1
+    assert float(other.slots()[1][0][5]) == top
+    for o in (opt, other):
+        o.apply_gradients(torch.zeros_like(grad))
+    finite = torch.arange(256, device='cuda') != 200
+    assert bool(other.slots()[1][0][finite].isfinite().all()) and bool(other._variables[0][finite].isfinite().all())
