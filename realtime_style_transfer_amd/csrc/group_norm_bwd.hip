@@ -13,6 +13,8 @@
 // slopes on the kinks: relu 0 at 0; hard_swish 0 at -3 and 1 at 3, where its forward's branches are.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "group_norm_device.h"
 
 namespace rst {
@@ -23,7 +25,11 @@ using namespace gn;
 // vectors of a batch per thread: 32 bytes of each tensor (hard_swish has too many constants for that beside them)
 template <typename T, int ACT>
 constexpr int U = ACT == HARD_SWISH ? 2 : 8 / (int)sizeof(T);
-constexpr int THREAD_PX = 64;                  // values that a thread sums in f32
+constexpr int THREAD_PX = 64;                  // values that a thread sums
+// A thread's sums: in 64 bits, and for bf16 tensors in 32: 64 values of 8 bits lose less there than their own rounding (1.5e-7
+// of the affine's gradients instead of 0.8e-7), and with 64 bits the registers spill (norm_grad_stem 101 us, so 116)
+template <typename T>
+using Sum = typename std::conditional<sizeof(T) == 4, double, float>::type;
 constexpr int MERGE_CHANNELS = 2048;
 // As the forward's, per workgroup of the second pass: one image of 28800 pixels, 128 channels (256 KB) 22.8 us (with the
 // launch 22.1, and 3 us more on the host), 256 channels x 14400 pixels (512 KB) 26.4 (22.1)
@@ -90,10 +96,11 @@ struct Channels {
         return dy;
     }
     // a value's share of the sums of dz and dz h (dz d, to be multiplied by rstd later, can pass f32)
-    __device__ __forceinline__ void add(float x, float dy, int i, float& s1, float& s2) const {
+    template <typename S>
+    __device__ __forceinline__ void add(float x, float dy, int i, S& s1, S& s2) const {
         const float d = x - mean[i], g = dz(x, d, dy, i);
-        s1 += g;
-        s2 = fmaf(g, d * rstd[i], s2);
+        s1 += (S)g;
+        s2 = fma((S)g, (S)(d * rstd[i]), s2);
     }
 };
 
@@ -132,9 +139,9 @@ template <typename T, int V, int ACT>
 __global__ __launch_bounds__(NT) void gn_bwd_stats_kernel(GroupNormArgs a, BwdParts p, Geom g, int block0) {
     __shared__ float2 red[NT * V];
     const Place w = place(g, blockIdx.x + block0);
-    float s1[V], s2[V];
+    Sum<T> s1[V], s2[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
+    for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0;
     if (w.active) {
         Walk<Pack<T, V>, 2, U<T, ACT>, false> walk;
         const void* in[2] = {a.x, a.dy};
@@ -147,7 +154,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_stats_kernel(GroupNormArgs a, BwdPa
         });
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = make_float2(s1[i], s2[i]);
+    for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = make_float2((float)s1[i], (float)s2[i]);
     __syncthreads();
     const int c0 = w.cb * g.nvb * V, width = min(g.C, c0 + g.nvb * V) - c0;
     float2* out = p.part + ((size_t)w.b * g.tiles + w.tile) * g.C + c0;
@@ -323,9 +330,9 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(GroupNormArgs a, doubl
     int b = all ? 0 : image;
     size_t at = ((size_t)b * u.hw + row) * u.nv + vec;
     Pack<T, V> x[R], dy[R];
-    float s1[V], s2[V];
+    Sum<T> s1[V], s2[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
+    for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0;
     Channels<ACT, V> k;
     if (active)
         for (;;) {
@@ -349,7 +356,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(GroupNormArgs a, doubl
             at += (size_t)u.hw * u.nv;
         }
 #pragma unroll
-    for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = make_float2(s1[i], s2[i]);
+    for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = make_float2((float)s1[i], (float)s2[i]);
     __syncthreads();
     const bool own = all || a.aff_stride != 0 || u.B == 1;
     column_sums(red, u.rows, u.bv * V, u.bv * V, u.threads, [&](int c, double2 s) __attribute__((always_inline)) {
