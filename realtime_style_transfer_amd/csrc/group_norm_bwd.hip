@@ -26,10 +26,11 @@ using namespace gn;
 template <typename T, int ACT>
 constexpr int U = ACT == HARD_SWISH ? 2 : 8 / (int)sizeof(T);
 constexpr int THREAD_PX = 64;                  // values that a thread sums
-// A thread's sums: in 64 bits, and for bf16 tensors in 32: 64 values of 8 bits lose less there than their own rounding (1.5e-7
-// of the affine's gradients instead of 0.8e-7), and with 64 bits the registers spill (norm_grad_stem 101 us, so 116)
-template <typename T>
-using Sum = typename std::conditional<sizeof(T) == 4, double, float>::type;
+// A thread's sums are in 64 bits. In the first pass of swish over bf16 tensors in 32: 64 values of 8 bits lose less there than by
+// their own rounding (the affine's gradients are off by 1.5e-7, in 64 bits by 0.8e-7), and in 64 bits the registers spill
+// (norm_grad_stem 101 us, so 116). Its cost elsewhere: 0 to 1 % (four activations, 1 to 118 MB)
+template <typename T, int ACT>
+using Sum = typename std::conditional<sizeof(T) == 2 && ACT == SWISH, float, double>::type;
 constexpr int MERGE_CHANNELS = 2048;
 // As the forward's, per workgroup of the second pass: one image of 28800 pixels, 128 channels (256 KB) 22.8 us (with the
 // launch 22.1, and 3 us more on the host), 256 channels x 14400 pixels (512 KB) 26.4 (22.1)
@@ -139,7 +140,7 @@ template <typename T, int V, int ACT>
 __global__ __launch_bounds__(NT) void gn_bwd_stats_kernel(GroupNormArgs a, BwdParts p, Geom g, int block0) {
     __shared__ float2 red[NT * V];
     const Place w = place(g, blockIdx.x + block0);
-    Sum<T> s1[V], s2[V];
+    Sum<T, ACT> s1[V], s2[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0;
     if (w.active) {
@@ -330,7 +331,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(GroupNormArgs a, doubl
     int b = all ? 0 : image;
     size_t at = ((size_t)b * u.hw + row) * u.nv + vec;
     Pack<T, V> x[R], dy[R];
-    Sum<T> s1[V], s2[V];
+    double s1[V], s2[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0;
     Channels<ACT, V> k;

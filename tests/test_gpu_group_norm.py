@@ -509,11 +509,12 @@ def test_gradients_of_activations_far_from_one(shape, size):
             _near(g, want, tol, f"{act} {what}")
 
 
-def test_sums_of_gradients_of_very_different_sizes():
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sums_of_gradients_of_very_different_sizes(dtype):
     """A 32nd of the pixels, those that threads meet first, has gradients of 2^25: added to one of them in 32 bits, the others'
     ones would be lost, 15 e of the sum. The threads' sums are in 64 bits: partials and the result are rounded, 2 e."""
     H, W = 4096, 4096
-    x, one = torch.ones(1, H, W, 4, device='cuda'), torch.ones(4, device='cuda')
+    x, one = torch.ones(1, H, W, 4, dtype=dtype, device='cuda'), torch.ones(4, device='cuda')
     dy = torch.ones_like(x)
     dy[:, :H // 32] = 2.0 ** 25
     dx, dscale, dbias = _op()[1](x, dy, one, 0 * one, torch.zeros(1, 2, device='cuda'), torch.ones(1, 2, device='cuda'), 2)
