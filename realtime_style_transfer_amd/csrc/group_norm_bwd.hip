@@ -26,9 +26,11 @@ using namespace gn;
 template <typename T, int ACT>
 constexpr int U = ACT == HARD_SWISH ? 2 : 8 / (int)sizeof(T);
 constexpr int THREAD_PX = 64;                  // values that a thread sums
-// A thread's sums are in 64 bits. In the first pass of swish over bf16 tensors in 32: 64 values of 8 bits lose less there than by
-// their own rounding (the affine's gradients are off by 1.5e-7, in 64 bits by 0.8e-7), and in 64 bits the registers spill
-// (norm_grad_stem 101 us, so 116). Its cost elsewhere: 0 to 1 % (four activations, 1 to 118 MB)
+// A thread's sums are in 64 bits in the first of two passes. In 32 where that would cost more than it gives: swish over bf16
+// tensors (64 values of 8 bits lose less by it than by their own rounding: the affine's gradients are off by 1.5e-7, in 64
+// bits by 0.8e-7; the registers would spill, norm_grad_stem 101 us, so 116), and the one launch, whose threads add up eight
+// values at most (in 64 bits its widest forms spill: 2048 pixels x 128 channels in groups of 16, relu 11.8 us, so 13.7,
+// hard_swish 17.2, so 21.0). Elsewhere it costs 0 to 1 % (four activations, 1 to 118 MB)
 template <typename T, int ACT>
 using Sum = typename std::conditional<sizeof(T) == 2 && ACT == SWISH, float, double>::type;
 constexpr int MERGE_CHANNELS = 2048;
@@ -134,8 +136,9 @@ __device__ __forceinline__ void column_sums(const float2* red, int rows, int wid
     }
 }
 
-// Pass 1. 118 + 118 MB bf16 with swish in 44 us (5.3 TB/s), 59 + 59 MB f32 with relu in 23 (5.1 TB/s): bound by reading;
-// swish's 14 instructions a value, two of them at half rate, would take 25 of the 44 by themselves
+// Pass 1. 118 + 118 MB bf16 with swish in 45 us (5.2 TB/s), 59 + 59 MB f32 with relu in 23 (5.1 TB/s): bound by reading;
+// swish's 17 instructions a value would take 26 of the 45 by themselves. Partials are rounded to f32, which halves what the
+// merges read: a large tensor has 200 of them or more, each off by half a step at most
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(NT) void gn_bwd_stats_kernel(GroupNormArgs a, BwdParts p, Geom g, int block0) {
     __shared__ float2 red[NT * V];
@@ -241,7 +244,7 @@ __device__ __forceinline__ void group_sums(const GroupNormArgs& a, int b, int g0
 }
 
 // Pass 2. MERGE: the image's sums are merged here, while the first loads are under way (one channel block only). Bound by
-// memory: 236 MB read, 118 MB written in 54 us (6.5 TB/s), 118 and 59 MB in 28.7 (6.2 TB/s)
+// memory: 236 MB read, 118 MB written in 55.7 us (6.4 TB/s), 118 and 59 MB in 28.9 (6.1 TB/s)
 template <typename T, int V, int ACT, bool MERGE, bool PAST>
 __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(GroupNormArgs a, BwdParts p, Geom g, int block0) {
     __shared__ double2 chan[MERGE ? MERGE_CHANNELS : 1];
@@ -331,9 +334,9 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(GroupNormArgs a, doubl
     int b = all ? 0 : image;
     size_t at = ((size_t)b * u.hw + row) * u.nv + vec;
     Pack<T, V> x[R], dy[R];
-    double s1[V], s2[V];
+    float s1[V], s2[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0;
+    for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
     Channels<ACT, V> k;
     if (active)
         for (;;) {
@@ -480,7 +483,8 @@ hipError_t backward_t(const GroupNormArgs& a, hipStream_t st) {
 
 template <typename T>
 hipError_t backward(const GroupNormArgs& a, hipStream_t st) {
-    // four channels at most: with eight, their constants (mean, rstd, scale, thresholds, ...) spill at 1024 threads
+    // four channels at most: with eight, their constants (mean, rstd, scale, thresholds, ...) spill at 1024 threads. (With four,
+    // hard_swish in the one-launch form of eight f32 vectors a thread does, 12 registers)
     switch (vector_width<T>((size_t)a.x | (size_t)a.dy | (size_t)a.out, a.C, 4)) {
         case 4: return backward_t<T, 4>(a, st);
         case 2: return backward_t<T, 2>(a, st);
