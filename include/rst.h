@@ -156,7 +156,7 @@ int rst_instance_norm(const float* x, int batch, int hw, int channels, const flo
  * runs on 16-byte loads; at most 2^27 channels, batch * channels below 2^31 - 648. y may be x. mean / rstd (B, groups)
  * receive the statistics when not NULL.
  * backward: from dy, x and the forward's mean / rstd: dx (may be dy), dscale and dbias shaped as scale / bias (sums over
- * the batch where they are shared). The same inputs give the same bits (no atomics). batch or hw 0: RST_OK, nothing is
+ * the batch where they are shared); relu's slope is 0 at 0, hard_swish's 0 up to -3 and 1 from 3 on. The same inputs give the same bits (no atomics). batch or hw 0: RST_OK, nothing is
  * written but dscale = dbias = 0. workspace: rst_group_norm(_backward)_workspace_size() bytes (0: may be NULL), aligned to
  * 16, used by one call at a time (calls on two streams, or two captured graphs that may replay together, need one each). */
 enum { RST_DTYPE_FLOAT32 = 0, RST_DTYPE_BFLOAT16 = 1 };

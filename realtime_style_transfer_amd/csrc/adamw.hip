@@ -12,7 +12,9 @@
 // nearest. v / s is rounded up or down at random with the right mean: (1 - b2) of a change is far below half a code, so
 // that rounding to nearest would leave v where it is for ever. The random bits are a hash of (element, step, seed), so
 // a step is reproducible. A v above zero keeps a code above zero: its root divides. Moments, scales and codes are
-// formed in 64 bits, which issue at the f32 rate here, so that a code does not depend on the order of operations.
+// formed in 64 bits, which issue at the f32 rate here, so that a code does not depend on the order of operations. The
+// variable's step itself is in 32 bits, about 10 units of 2^-24 of it: learning_rate times that is far below the rounding of
+// the variable.
 #include <hip/hip_runtime.h>
 
 #include "adamw.h"
@@ -81,7 +83,7 @@ __global__ __launch_bounds__(ADAMW_PTRS) void set_pointers_kernel(AdamwPtrs p, c
 }
 
 // Sums of squares over the chunks blockIdx, blockIdx + grid, ...: one partial per workgroup, merged by the step. 192 MB in
-// 31 us (6.2 TB/s: reading bound), 11 MB in 4.5
+// 32 us (6.0 TB/s: reading bound), 11 MB in 4.6
 template <bool BF16>
 __global__ __launch_bounds__(NT) void norm_kernel(AdamwArgs a, double* partials) {
     __shared__ double red[4];
@@ -205,8 +207,8 @@ __device__ __forceinline__ void adamw_elements(const float (&g)[N], float (&p)[N
     for (int k = 0; k < N; ++k) p[k] = fmaf(-s.lr, fmaf(s.decay, p[k], q[k]), p[k]);
 }
 
-// Bound by memory: 48 M elements with bf16 gradients, 1.25 GB, in 214 us (5.8 TB/s; torch's copy of 1 GiB 5.1), 2.7 M
-// elements in 13.6 (their 76 MB stay in the Infinity Cache). Every load of a thread comes before the first use, the step's
+// Bound by memory: 48 M elements with bf16 gradients, 1.25 GB, in 216 us (5.8 TB/s; torch's copy of 1 GiB 5.1), 2.7 M
+// elements in 13.7 (their 76 MB stay in the Infinity Cache). Every load of a thread comes before the first use, the step's
 // scalars in between
 template <bool BF16, bool PAST>
 __global__ __launch_bounds__(NT) void adamw32_kernel(AdamwArgs a) {
@@ -278,7 +280,7 @@ __global__ __launch_bounds__(NT) void adamw32_kernel(AdamwArgs a) {
 
 // ---- 8-bit states --------------------------------------------------------------------------------------------------
 
-// Two rounds of xor-shift and multiply: a bijection of 32 bits whose outputs look random
+// Two rounds of xor-shift and multiply, a bijection of 32 bits whose outputs look random: the published integer hash lowbias32
 __device__ __forceinline__ unsigned mix(unsigned x) {
     x = (x ^ (x >> 16)) * 0x7FEB352Du;
     x = (x ^ (x >> 15)) * 0x846CA68Bu;
@@ -444,8 +446,9 @@ __device__ __forceinline__ void step8(Eight& e, const AdamwArgs& a, const AdamwC
 }
 
 // Eight elements per lane and round: a chunk is at most two rounds. Bound by memory with about 50 instructions an element
-// beside it: 48 M elements, 774 MB, in 147 us (5.3 TB/s); 61 k elements in 5.0, latency. (Three waves per SIMD: at four
-// the registers spill, 12 M elements 51 us for 48)
+// beside it: 48 M elements, 774 MB, in 147 to 158 us (from card to card; 4.9 to 5.3 TB/s); 61 k elements in 4.8, latency; 2.7 M in 13.1,
+// with clipping 14.5: each of its 1537 workgroups then merges the norm's partial sums by itself, 8 KB, before its first
+// element. (Three waves per SIMD: at four the registers spill, 12 M elements 51 us for 48)
 template <bool BF16, bool PAST>
 __global__ __launch_bounds__(NT, 3) void adamw8_kernel(AdamwArgs a) {
     __shared__ double red[4];

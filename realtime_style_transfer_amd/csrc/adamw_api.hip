@@ -30,8 +30,8 @@ struct rst_adamw {
 
 namespace {
 
-// A step that touches more than half of the 256 MB Infinity Cache loads and stores past it (12 M elements, 32-bit states
-// 70 us, through it 80; 6 M 38.9 and 44.4)
+// A step that touches more than half of the 256 MB Infinity Cache loads and stores past it (with the larger chunks and 32-bit
+// states, 12 M elements 70 us, through it 80; 6 M 38.9 and 44.4)
 constexpr size_t STREAMING_BYTES = 128u << 20;
 constexpr size_t MAX_CHUNKS = 0xFFFFFFFFu / 256;     // HIP launches fewer than 2^32 threads, 256 of them a chunk's
 // The kernels take the reciprocal of sqrt(v) + epsilon in f32: below 2^-126 it is infinite, and an element with m = v = 0 a NaN

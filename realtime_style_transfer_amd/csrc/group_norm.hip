@@ -77,7 +77,7 @@ __device__ __forceinline__ void add_moments(const Pack<T, V>& v, double* s, doub
     }
 }
 
-// Pass 1: sums of x and x^2 of every (image, group) over a tile. Bound by reading x: 59 MB bf16 in 12.1 us (4.9 TB/s),
+// Pass 1: sums of x and x^2 of every (image, group) over a tile. Bound by reading x: 59 MB bf16 in 11.9 us (5.0 TB/s),
 // 236 MB f32 in 40.6 (5.8 TB/s; a kernel that only reads: 6.4)
 template <typename T, int V, bool UNI>
 __global__ __launch_bounds__(NT) void gn_stats_kernel(const void* x, Parts parts, Geom g, int block0) {
@@ -157,8 +157,10 @@ __global__ __launch_bounds__(256) void gn_finalize_kernel(Parts p, float* mean, 
 }
 
 // Pass 2: y = act(a x + c). MERGE: the image's sums are merged here, while the first loads are under way. Bound by memory:
-// 59 + 59 MB bf16 in 20.8 us (5.7 TB/s), 236 + 236 MB f32 past the caches in 69 (6.8 TB/s: x comes from the Infinity
-// Cache). 32-bit arithmetic instead of the f64 FMA was no faster (20.9, 68)
+// 59 + 59 MB bf16 in 21 us (5.6 TB/s), 236 + 236 MB f32 stored past the caches in 68 (7.0 TB/s: more than HBM gives, so some
+// of x comes from the Infinity Cache; all of it comes from behind L2). 32-bit arithmetic instead of the f64 FMA was no
+// faster. One image has less of both than of the merge's: 28800 pixels x 128 channels f32 are 14.7 MB, and each of the 225
+// workgroups merges 115 KB of sums, 26 MB in all, which L2 holds (8.2 us)
 constexpr int MERGE_GROUPS = 1024;
 template <typename T, int V, int ACT, bool MERGE, bool PAST>
 __global__ __launch_bounds__(NT) void gn_apply_kernel(GroupNormArgs a, Parts p, Geom g, int block0) {
@@ -215,7 +217,7 @@ __global__ __launch_bounds__(NT) void gn_apply_kernel(GroupNormArgs a, Parts p, 
 }
 
 // One launch: the bundle's values stay in registers between the moments and the output. Bound by latency: 450 pixels x 96
-// channels 6.1 us, an almost empty image 3.6 in a graph
+// channels 6.1 us, an almost empty image 3.6 in a graph. (The widest form, bf16 with 16 vectors of eight, spills 8 registers)
 template <typename T, int V, bool UNI, int R>
 __global__ __launch_bounds__(NT) void gn_fused_kernel(GroupNormArgs a, Bundle u, int block0) {
     constexpr int E = UNI ? 1 : V;

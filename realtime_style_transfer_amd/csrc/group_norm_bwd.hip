@@ -28,7 +28,7 @@ constexpr int U = ACT == HARD_SWISH ? 2 : 8 / (int)sizeof(T);
 constexpr int THREAD_PX = 64;                  // values that a thread sums
 // A thread's sums are in 64 bits in the first of two passes. In 32 where that would cost more than it gives: swish over bf16
 // tensors (64 values of 8 bits lose less by it than by their own rounding: the affine's gradients are off by 1.5e-7, in 64
-// bits by 0.8e-7; the registers would spill, norm_grad_stem 101 us, so 116), and the one launch, whose threads add up eight
+// bits by 0.8e-7; the registers would spill, 4 x 480 x 960 x 32 101 us, so 116), and the one launch, whose threads add up eight
 // values at most (in 64 bits its widest forms spill: 2048 pixels x 128 channels in groups of 16, relu 11.8 us, so 13.7,
 // hard_swish 17.2, so 21.0). Elsewhere it costs 0 to 1 % (four activations, 1 to 118 MB)
 template <typename T, int ACT>

@@ -376,7 +376,8 @@ def group_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, groups:
 def group_norm_gradients(x: torch.Tensor, dy: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, mean: torch.Tensor,
                          rstd: torch.Tensor, groups: int, activation: str = "linear"):
     """The gradients of ``group_norm``: from dy = d loss / d y (like x) and the forward's statistics -> (dx like x, dscale,
-    dbias shaped as scale; sums over the batch where the affine is shared)."""
+    dbias shaped as scale; sums over the batch where the affine is shared). On its kinks an activation's slope is 0 (relu at
+    0, hard_swish at -3) or 1 (hard_swish at 3)."""
     dtype, act, per_image, B, HW, C, _, need = _group_norm_plan(x.shape, x.dtype, scale.shape, bias.shape, groups,
                                                                 activation)
     index = _group_norm_tensors(x, scale, bias, dy, mean, rstd)
