@@ -156,9 +156,10 @@ int rst_instance_norm(const float* x, int batch, int hw, int channels, const flo
  * runs on 16-byte loads; at most 2^27 channels, batch * channels below 2^31 - 648. y may be x. mean / rstd (B, groups)
  * receive the statistics when not NULL.
  * backward: from dy, x and the forward's mean / rstd: dx (may be dy), dscale and dbias shaped as scale / bias (sums over
- * the batch where they are shared); relu's slope is 0 at 0, hard_swish's 0 up to -3 and 1 from 3 on. The same inputs give the same bits (no atomics). batch or hw 0: RST_OK, nothing is
- * written but dscale = dbias = 0. workspace: rst_group_norm(_backward)_workspace_size() bytes (0: may be NULL), aligned to
- * 16, used by one call at a time (calls on two streams, or two captured graphs that may replay together, need one each). */
+ * the batch where they are shared); relu's slope is 0 at 0, hard_swish's 0 up to -3 and 1 from 3 on. The same inputs give
+ * the same bits (no atomics). batch or hw 0: RST_OK, nothing is written but dscale = dbias = 0. workspace:
+ * rst_group_norm(_backward)_workspace_size() bytes (0: may be NULL), aligned to 16, used by one call at a time (calls on
+ * two streams, or two captured graphs that may replay together, need one each). */
 enum { RST_DTYPE_FLOAT32 = 0, RST_DTYPE_BFLOAT16 = 1 };
 enum { RST_ACT_LINEAR = 0, RST_ACT_RELU = 1, RST_ACT_SWISH = 2, RST_ACT_HARD_SWISH = 3 };
 size_t rst_group_norm_workspace_size(int batch, int hw, int channels, int groups);
@@ -361,7 +362,8 @@ int rst_predictor_trainer_set_moving_statistics(rst_predictor_trainer* t, const 
  *   global_norm: receives |g| of each step that clips (may be NULL). If |g| is not finite that step changes nothing,
  *     iterations included. Without clipping a NaN or an infinity stays with its element, whose moments are NaN then (a
  *     NaN code, which counts for no scale); a v beyond 448 times f32's largest value saturates.
- * States start as zeros (iterations 0). A captured step needs the handle for as long as it replays. One step of a handle at a time: not on two streams at once. */
+ * States start as zeros (iterations 0). A captured step needs the handle for as long as it replays. One step of a handle at a
+ * time: not on two streams at once. */
 typedef struct rst_adamw_tensor {
     float* param;
     size_t count;

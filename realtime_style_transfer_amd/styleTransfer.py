@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import logging
+import operator
 from typing import Dict, List, Optional, Sequence
 
 import numpy as np
@@ -353,6 +354,7 @@ def group_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, groups:
     x (B,H,W,C) float32 or bfloat16; scale and bias (C,), or (B,C) per image (style parameters), float32; activation
     "linear", "relu", "swish" or "hard_swish". groups == C is ``instance_norm``. Returns y like x; with
     ``return_statistics`` (y, mean, rstd), the statistics (B, groups) float32 that ``group_norm_gradients`` takes."""
+    groups, eps = operator.index(groups), float(eps)
     dtype, act, per_image, B, HW, C, need, _ = _group_norm_plan(x.shape, x.dtype, scale.shape, bias.shape, groups,
                                                                 activation)
     index = _group_norm_tensors(x, scale, bias)
@@ -378,6 +380,7 @@ def group_norm_gradients(x: torch.Tensor, dy: torch.Tensor, scale: torch.Tensor,
     """The gradients of ``group_norm``: from dy = d loss / d y (like x) and the forward's statistics -> (dx like x, dscale,
     dbias shaped as scale; sums over the batch where the affine is shared). On its kinks an activation's slope is 0 (relu at
     0, hard_swish at -3) or 1 (hard_swish at 3)."""
+    groups = operator.index(groups)
     dtype, act, per_image, B, HW, C, _, need = _group_norm_plan(x.shape, x.dtype, scale.shape, bias.shape, groups,
                                                                 activation)
     index = _group_norm_tensors(x, scale, bias, dy, mean, rstd)

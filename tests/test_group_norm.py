@@ -111,3 +111,16 @@ def test_sizes_past_the_interface_are_refused():
     for shape in ((1, 2 ** 16, 2 ** 16, 1), (2 ** 31, 1, 1, 1)):
         with pytest.raises(ValueError, match="2\\^31"):
             group_norm(torch.empty(shape, dtype=torch.bfloat16, device='meta'), s, s, 1)
+
+
+def test_numbers_of_other_kinds():
+    """Groups as any whole number, eps as any real one; a group count of 2.0 is none."""
+    x, s, st = torch.zeros(2, 3, 5, 14), torch.ones(14), torch.zeros(2, 7)
+    for groups, eps in ((np.int64(7), np.float32(1e-5)), (torch.tensor(7), torch.tensor(1e-5))):
+        with pytest.raises(ValueError, match="CPU tensor"):
+            group_norm(x, s, s, groups, eps=eps)
+        with pytest.raises(ValueError, match="CPU tensor"):
+            group_norm_gradients(x, x, s, s, st, st, groups)
+    for call in (lambda: group_norm(x, s, s, 7.0), lambda: group_norm_gradients(x, x, s, s, st, st, 7.0)):
+        with pytest.raises(TypeError):
+            call()
